@@ -100,7 +100,8 @@ enum {
     SFB_STATUS_BAD_BLOCK_ID = 1, /* block-table entry outside [0, NB): block skipped */
     SFB_STATUS_EMPTY_REQUEST = 2, /* seq_len <= 0: output row zero-filled */
     SFB_STATUS_WAIT_TIMEOUT = 4, /* a bounded device-side wait gave up */
-    SFB_STATUS_UNSORTED_POSITIONS = 8 /* sfb_attention_dense: a positional mask whose positions decrease somewhere */
+    SFB_STATUS_UNSORTED_POSITIONS = 8, /* sfb_attention_dense: a positional mask whose positions decrease somewhere */
+    SFB_STATUS_BAD_ROW_INDEX = 16 /* group offsets that decrease or leave the rows, a row index or position outside: see each call */
 };
 
 SFB_API int sfb_abi_version(void);
@@ -454,6 +455,57 @@ SFB_API int sfb_fused_rms_norm_matmul_plan(int64_t rows, int64_t cols, int sms, 
 SFB_API int sfb_fold_norm_weight(const SFBTensor* rms_weight, const SFBTensor* mat_weight, SFBTensor* folded, int dtype, void* stream);
 SFB_API int sfb_fused_rms_norm_matmul(const SFBTensor* x, const SFBTensor* folded_weight, SFBTensor* out, int dtype, float eps,
                                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ── The feed-forward half of a decoder layer ────────────────────────────────
+ * Dense product with its epilogue, the same product for rows grouped by expert, the router
+ * in front of it and the weighted sum behind it.  `status` (device int32, may be NULL)
+ * collects status bits with atomic ORs; the caller clears it. */
+enum { SFB_ACT_NONE = 0, SFB_ACT_SILU = 1, SFB_ACT_GELU = 2 /* erf */, SFB_ACT_GELU_TANH = 3, SFB_ACT_RELU = 4 };
+enum { SFB_WEIGHT_KN = 0, /* [.., K, N], N contiguous */ SFB_WEIGHT_NK = 1 /* [.., N, K], K contiguous: as checkpoints store a projection */ };
+
+/*   out = act(x W + bias) * (x V + up_bias) + residual
+ *   x [M, K]  weight [K, N] or [N, K] (weight_layout)  bias [N] or NULL
+ *   up_weight (V) like weight, or NULL: then the second factor is left out;  up_bias [N] or NULL (needs up_weight)
+ *   residual [M, N] in out_dtype or NULL; it may be `out` itself
+ *   out [M, N] in out_dtype: dtype or F32.  dtype: F32, BF16, F16
+ * Products and sums in fp32 (16-bit products are exact there), one rounding of the result.  bf16 / fp16 operands whose
+ * bases and row strides are multiples of 16 bytes run on the tensor cores; every other type, alignment and stride on
+ * the CUDA cores. */
+SFB_API int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight, const SFBTensor* up_bias,
+                             const SFBTensor* residual, SFBTensor* out, int weight_layout, int dtype, int out_dtype, int activation, int32_t* status,
+                             void* stream);
+
+/* Rows r of out with group_offsets[e] <= r < group_offsets[e + 1] are act(x[i] W[e] + bias[e]) * (x[i] V[e] + up_bias[e]),
+ * i = row_index[r], or r without a row_index.
+ *   x [X, K]  weight, up_weight [E, K, N] or [E, N, K]  bias, up_bias [E, N] or NULL
+ *   group_offsets int32 [E + 1], read on the device: not decreasing, within 0 .. R; groups may be empty
+ *   row_index int32 [R] or NULL  out [R, N]
+ * Rows of out outside every group are left as they were.  E <= 1024.  Offsets that leave 0 .. R are clamped, a
+ * decreasing pair is an empty group, and a row index outside 0 .. X-1 reads row 0; each sets SFB_STATUS_BAD_ROW_INDEX. */
+SFB_API int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight,
+                               const SFBTensor* up_bias, const SFBTensor* group_offsets, const SFBTensor* row_index, SFBTensor* out,
+                               int weight_layout, int dtype, int out_dtype, int activation, int32_t* status, void* stream);
+
+/* The top_k experts of every token and the assignments sorted by expert.
+ *   logits [T, E] (F32 | BF16 | F16), E <= 1024; top_k <= min(E, 32)
+ *   expert_ids int32, weights float32, positions int32, each [T, top_k] contiguous;
+ *   group_offsets int32 [E + 1]; token_rows int32 [T * top_k]
+ * A token's experts come in the order larger logit first, then lower index; a logit of -inf or NaN never chooses its
+ * expert, and a token with fewer than top_k candidates has id -1, weight 0 and position -1 in the places left over.
+ * weights: softmax over the chosen experts (renormalize) or over all E.  Assignment (t, j) is row positions[t, j] of the
+ * sorted order, token_rows[row] = t, rows of expert e are group_offsets[e] .. group_offsets[e + 1] in the order of
+ * tokens; token_rows behind the last row is -1.  (logits of +inf share the weight among themselves.)
+ * workspace: sfb_moe_route_workspace_bytes(T, E) bytes, 0 for few tokens; its contents need not be kept. */
+SFB_API int64_t sfb_moe_route_workspace_bytes(int64_t tokens, int64_t experts);
+SFB_API int sfb_moe_route(const SFBTensor* logits, SFBTensor* expert_ids, SFBTensor* weights, SFBTensor* group_offsets, SFBTensor* token_rows,
+                          SFBTensor* positions, int dtype, int renormalize, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[t, :] = sum over j of weights[t, j] y[positions[t, j], :]  + residual[t, :]
+ *   y [R, H]  positions int32, weights float32 [T, k], k <= 32  residual, out [T, H] (residual may be NULL or `out` itself)
+ * dtype F32, BF16 or F16 for y, residual and out; fp32 sums in the order of j, one rounding.  Position -1 adds nothing;
+ * any other position outside 0 .. R-1 adds nothing either and sets SFB_STATUS_BAD_ROW_INDEX. */
+SFB_API int sfb_moe_combine(const SFBTensor* y, const SFBTensor* positions, const SFBTensor* weights, const SFBTensor* residual, SFBTensor* out,
+                            int dtype, int32_t* status, void* stream);
 
 /* ── `_mlir_ciface_*` convention ─────────────────────────────────────────────
  * The reference's runtime calls compiled kernels as

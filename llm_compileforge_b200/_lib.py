@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, Structure, Union, byref, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
@@ -35,6 +36,9 @@ SFB_F32, SFB_BF16, SFB_F16, SFB_F8E4M3 = 0, 1, 2, 3
 SFB_QUANT_PER_TENSOR, SFB_QUANT_PER_BLOCK_HEAD = 0, 1
 
 SFB_STATUS_BAD_BLOCK_ID, SFB_STATUS_EMPTY_REQUEST, SFB_STATUS_WAIT_TIMEOUT, SFB_STATUS_UNSORTED_POSITIONS = 1, 2, 4, 8
+SFB_STATUS_BAD_ROW_INDEX = 16
+SFB_ACT_NONE, SFB_ACT_SILU, SFB_ACT_GELU, SFB_ACT_GELU_TANH, SFB_ACT_RELU = 0, 1, 2, 3, 4
+SFB_WEIGHT_KN, SFB_WEIGHT_NK = 0, 1
 SFB_MASK_NONE, SFB_MASK_CAUSAL_TOP_LEFT, SFB_MASK_CAUSAL_BOTTOM_RIGHT, SFB_MASK_POSITIONS = 0, 1, 2, 3
 
 _DTYPES = {
@@ -116,6 +120,7 @@ def load() -> ctypes.CDLL:
     _optional(lib)
     _shared_prefix_protos(lib)
     _block_manager_protos(lib)
+    _feed_forward_protos(lib)
     lib.sfb_paged_attention_decode_gather.restype = c_int
     lib.sfb_paged_attention_decode_gather.argtypes = [_T] * 9 + [POINTER(c_void_p), c_int, c_int, c_int, c_int, c_float, c_int64,
                                                                 c_void_p, c_int64, c_void_p]
@@ -186,6 +191,20 @@ def _shared_prefix_protos(lib: ctypes.CDLL) -> None:
     lib.sfb_paged_attention_decode_shared_prefix.argtypes = [_T] * 6 + [c_int, c_float, c_int64, c_int64, c_void_p, c_int64, c_void_p]
 
 
+def _feed_forward_protos(lib: ctypes.CDLL) -> None:
+    t = c_void_p  # descriptors as bytes (see :func:`packed`)
+    lib.sfb_fused_linear.restype = c_int
+    lib.sfb_fused_linear.argtypes = [t] * 7 + [c_int] * 4 + [c_void_p, c_void_p]
+    lib.sfb_grouped_linear.restype = c_int
+    lib.sfb_grouped_linear.argtypes = [t] * 8 + [c_int] * 4 + [c_void_p, c_void_p]
+    lib.sfb_moe_route_workspace_bytes.restype = c_int64
+    lib.sfb_moe_route_workspace_bytes.argtypes = [c_int64, c_int64]
+    lib.sfb_moe_route.restype = c_int
+    lib.sfb_moe_route.argtypes = [t] * 6 + [c_int, c_int, c_void_p, c_int64, c_void_p]
+    lib.sfb_moe_combine.restype = c_int
+    lib.sfb_moe_combine.argtypes = [t] * 5 + [c_int, c_void_p, c_void_p]
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DTYPES[dtype]
@@ -216,6 +235,23 @@ def desc(t: torch.Tensor | None, what: str = "tensor"):
         raw.sizes[i] = t.shape[i]
         raw.strides[i] = t.stride(i)
     return byref(d)
+
+
+_PACK = [None] + [struct.Struct("=iiii2Qq%dq" % (2 * r)).pack for r in (1, 2, 3, 4)]
+
+
+def packed(t: torch.Tensor | None, what: str, device: torch.device):
+    """The descriptor of :func:`desc` as bytes (``None`` stays ``None``), for calls where a few microseconds of host time
+    count; the tensor must live on ``device``, a CUDA device."""
+    if t is None:
+        return None
+    if t.device != device or not t.is_cuda:
+        raise ValueError(f"{what} must live on {device if device.type == 'cuda' else 'a CUDA device'} (libsfb has no CPU path), got {t.device}")
+    shape = t.shape
+    if not 1 <= len(shape) <= 4:
+        raise ValueError(f"{what}: rank {len(shape)} outside 1..4")
+    p = t.data_ptr()
+    return _PACK[len(shape)](SFB_DEVICE_CUDA, len(shape), t.element_size(), 0, p, p, 0, *shape, *t.stride())
 
 
 def check(status: int) -> None:

@@ -1,0 +1,86 @@
+// Dense and grouped matrix products with an epilogue, expert routing and combining: launch arguments and what the
+// kernels share.
+#pragma once
+
+#include "sfb_common.cuh"
+
+namespace sfb {
+
+// out[r, n] = act(sum_k x[i, k] w[e, k, n] + bias[e, n]) * (sum_k x[i, k] up[e, k, n] + up_bias[e, n]) + residual[r, n]
+// for the rows r of group e, offsets[e] <= r < offsets[e + 1], with i = row_index[r] (or r).  Every part but the first
+// product may be missing; without offsets all rows are group 0.
+struct LinearArgs {
+    const void *x, *w, *up, *bias, *up_bias, *residual;
+    void* out;
+    const int32_t* offsets;    // [groups + 1] or nullptr
+    const int32_t* row_index;  // [rows] or nullptr
+    int64_t x_stride, out_stride, res_stride;  // elements between rows
+    int64_t w_stride[3], up_stride[3];         // group, k, n
+    int64_t bias_stride, up_bias_stride;       // group
+    int64_t rows, x_rows, K, N, groups;
+    int dtype, out_dtype, act;
+    int* status;
+};
+int launch_linear_generic(const LinearArgs& a, cudaStream_t stream);
+
+constexpr int kMaxGroups = 1024;  // groups (experts) of one call
+constexpr int kMaxTopK = 32;
+
+struct RouteArgs {
+    const void* logits;
+    int64_t logits_stride;
+    int32_t* ids;          // [T, k]
+    float* weights;        // [T, k]
+    int32_t* offsets;      // [E + 1]
+    int32_t* token_rows;   // [T k]
+    int32_t* positions;    // [T, k]
+    int32_t* counts;       // [blocks, E] scratch
+    int64_t tokens;
+    int experts, top_k, renormalize, dtype;
+};
+constexpr int kRouteTokens = 128;  // tokens of one thread block
+int launch_moe_route(const RouteArgs& a, cudaStream_t stream);
+
+struct CombineArgs {
+    const void *y, *residual;
+    const int32_t* positions;
+    const float* weights;
+    void* out;
+    int64_t y_stride, res_stride, out_stride, pos_stride, weight_stride;
+    int64_t tokens, y_rows, hidden;
+    int top_k, dtype;
+    int* status;
+};
+int launch_moe_combine(const CombineArgs& a, cudaStream_t stream);
+
+#ifdef __CUDACC__
+// Rows [begin, end) of group e.  Offsets come from the device and are not trusted: both ends are clamped to [0, rows]
+// and a pair that decreases is an empty group, so no address follows from a bad one.
+__device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int rows) {
+    const int b = offsets[e], t = offsets[e + 1];
+    const int lo = min(max(b, 0), rows);
+    return make_int2(lo, max(lo, min(max(t, 0), rows)));
+}
+
+// The activations in fp32.  silu and the tanh form of gelu as h * logistic(.), the erf form as h/2 * erfc(-h / sqrt 2):
+// none of them subtracts nearly equal numbers for large negative h.
+template <int ACT>
+__device__ __forceinline__ float activate(float h) {
+    if constexpr (ACT == SFB_ACT_SILU) return h / (1.f + __expf(-h));
+    if constexpr (ACT == SFB_ACT_GELU) return 0.5f * h * erfcf(-0.70710678118654752f * h);
+    if constexpr (ACT == SFB_ACT_GELU_TANH) return h / (1.f + __expf(-1.5957691216057308f * (h + 0.044715f * h * h * h)));
+    if constexpr (ACT == SFB_ACT_RELU) return h < 0.f ? 0.f : h;
+    return h;
+}
+__device__ __forceinline__ float activate(float h, int act) {
+    switch (act) {
+        case SFB_ACT_SILU: return activate<SFB_ACT_SILU>(h);
+        case SFB_ACT_GELU: return activate<SFB_ACT_GELU>(h);
+        case SFB_ACT_GELU_TANH: return activate<SFB_ACT_GELU_TANH>(h);
+        case SFB_ACT_RELU: return activate<SFB_ACT_RELU>(h);
+        default: return h;
+    }
+}
+#endif
+
+}  // namespace sfb

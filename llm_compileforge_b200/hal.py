@@ -70,6 +70,10 @@ class B200Backend(OpExecutor):
             "scaled_dot_product_attention": self._op_scaled_dot_product_attention,
             "chunked_prefill": self._op_chunked_prefill,
             "fused_rms_norm_matmul": self._op_fused_rms_norm_matmul,
+            "fused_linear": self._op_fused_linear,
+            "grouped_linear": self._op_grouped_linear,
+            "moe_route": self._op_moe_route,
+            "moe_combine": self._op_moe_combine,
         }
         self._folded: dict[tuple, torch.Tensor] = {}
 
@@ -247,6 +251,22 @@ class B200Backend(OpExecutor):
             # would then match the key with different contents
             entry = self._folded[key] = (ops.fold_norm_weight(g.contiguous(), w), g, w)
         return ops.fused_rms_norm_matmul(x, entry[0], eps=kw.get("eps", 1e-5))
+
+    def _op_fused_linear(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        """inputs ``[x, weight(, bias)]`` with the keywords of :func:`ops.fused_linear`."""
+        return ops.fused_linear(*inputs[:3], **kw)
+
+    def _op_grouped_linear(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        """inputs ``[x, weight, group_offsets(, bias)]`` with the keywords of :func:`ops.grouped_linear`."""
+        return ops.grouped_linear(*inputs[:4], **kw)
+
+    def _op_moe_route(self, inputs: list[Any], **kw: Any) -> Any:
+        """inputs ``[logits]`` with ``top_k`` and the keywords of :func:`ops.moe_route`."""
+        return ops.moe_route(inputs[0], kw.pop("top_k"), **kw)
+
+    def _op_moe_combine(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        """inputs ``[y, positions, weights]`` with the keywords of :func:`ops.moe_combine`."""
+        return ops.moe_combine(*inputs[:3], **kw)
 
     def _op_chunked_prefill(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[query [T,H,D], key_cache, value_cache, block_table [R,max_blocks]]``

@@ -8,10 +8,12 @@ dict-based signatures of the reference's ``kernels`` package are in
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
-from ._lib import check, current_stream, desc, dtype_code
+from ._lib import check, current_stream, desc, dtype_code, packed
 
 BLOCK_SIZE = 16
 
@@ -450,3 +452,199 @@ def norm_matmul_plan(rows: int, cols: int, *, sms: int = 148, clusters: int = 74
     check(_lib.load().sfb_fused_rms_norm_matmul_plan(int(rows), int(cols), int(sms), int(clusters), int(bool(has_workspace)), out))
     keys = ("pair", "tile_n", "stages", "k_steps_per_stage", "prepass", "x_box_rows")
     return dict(zip(keys, (int(v) for v in out)))
+
+
+# ── the feed-forward half of a decoder layer ────────────────────────────────
+ACTIVATIONS = {"none": _lib.SFB_ACT_NONE, "silu": _lib.SFB_ACT_SILU, "gelu": _lib.SFB_ACT_GELU, "gelu_tanh": _lib.SFB_ACT_GELU_TANH,
+               "relu": _lib.SFB_ACT_RELU}
+
+
+def _on(device: torch.device, fn, *args) -> None:
+    """One library call with ``device`` current (a launch needs its stream's device to be)."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, current_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, current_stream(device)))
+
+
+def _same_type(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+
+
+def _matrix(what: str, w: torch.Tensor, like: int | None = None) -> tuple[torch.Tensor, int]:
+    """A ``[.., K, N]`` weight as the library takes it: itself, or, when K is the contiguous dimension, its transpose."""
+    if w.stride(-1) == 1 and like != _lib.SFB_WEIGHT_NK:
+        return w, _lib.SFB_WEIGHT_KN
+    if w.stride(-2) == 1 and like != _lib.SFB_WEIGHT_KN:
+        return w.transpose(-1, -2), _lib.SFB_WEIGHT_NK
+    raise ValueError(f"{what}: one of the last two dimensions of a weight must be contiguous, the same one for both weights")
+
+
+def _rows(what: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    """``t [.., n]`` as rows that are written in place."""
+    if t.shape[-1:] != (n,):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, its last dimension must be {n}")
+    if t.dim() == 2:
+        return t
+    try:
+        return t.view(-1, n)
+    except RuntimeError:
+        raise ValueError(f"{what}: strides {t.stride()} do not make rows of {n}") from None
+
+
+def _activation(what: str, name: str) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what}: activation {name!r} not in {sorted(ACTIVATIONS)}") from None
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
+                 up_weight: torch.Tensor | None = None, up_bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight + bias) * (x @ up_weight + up_bias) + residual`` in one launch; every part but the first product is
+    optional.  ``x [..., K]``, ``weight`` and ``up_weight`` ``[K, N]`` with either dimension contiguous (a checkpoint's
+    ``[N, K]`` matrix goes in as its ``.t()`` view), ``residual [..., N]`` in the result's type.  ``activation``: one of
+    :data:`ACTIVATIONS`.  The result has ``x``'s type, or float32 with ``out_dtype=torch.float32``; ``out`` may be the residual
+    itself.  fp32 accumulation, one rounding.  bf16 / fp16 operands whose rows are 16-byte aligned run on the tensor
+    cores, all others on the CUDA cores.  ``status`` (int32, device) collects status bits."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"fused_linear: x [..., K] and weight [K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    k, n = weight.shape
+    act = _activation("fused_linear", activation)
+    odt = out.dtype if out is not None else out_dtype or x.dtype
+    _same_type("fused_linear", x.dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
+    _same_type("fused_linear", odt, residual=residual)
+    if k == 0:
+        raise ValueError("fused_linear: K is zero")
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.stride(-1) != 1 and k > 1:
+        x2 = x2.contiguous()
+    w, layout = _matrix("fused_linear", weight)
+    u = _matrix("fused_linear", up_weight, layout)[0] if up_weight is not None else None
+    shape = (*x.shape[:-1], n)
+    for name, t in (("out", out), ("residual", residual)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"fused_linear: {name} has shape {tuple(t.shape)}, expected {shape}")
+    if n == 0:
+        return torch.empty(shape, dtype=odt, device=x.device) if out is None else out
+    o2 = torch.empty((x2.shape[0], n), dtype=odt, device=x.device) if out is None else _rows("fused_linear: out", out, n)
+    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, n)
+    if r2 is not None and r2.stride(-1) != 1 and n > 1:
+        r2 = r2.contiguous()
+    dev = x.device
+    _on(dev, _lib.load().sfb_fused_linear, packed(x2, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
+        packed(up_bias, "up_bias", dev), packed(r2, "residual", dev), packed(o2, "out", dev), layout, dtype_code(x.dtype), dtype_code(odt), act,
+        _status_ptr(status, dev))
+    return out if out is not None else o2.view(shape)
+
+
+def _status_ptr(status: torch.Tensor | None, device: torch.device) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.device != device or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on {device}")
+    return status.data_ptr()
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.Tensor, bias: torch.Tensor | None = None, *,
+                   activation: str = "none", up_weight: torch.Tensor | None = None, up_bias: torch.Tensor | None = None,
+                   row_index: torch.Tensor | None = None, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                   status: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`fused_linear` for rows grouped by expert: row ``r`` with ``group_offsets[e] <= r < group_offsets[e + 1]`` (int32
+    ``[E + 1]``, read on the device, groups may be empty) is ``act(x[i] @ weight[e] + bias[e]) * (x[i] @ up_weight[e] + up_bias[e])``
+    with ``i = row_index[r]`` (int32, one entry per row of the result) or ``i = r`` without one.  ``weight`` and ``up_weight``
+    ``[E, K, N]`` with either of the last two dimensions contiguous, biases ``[E, N]``.  Rows outside every group are left as
+    they were (in a fresh result: undefined).  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
+    indices outside their range."""
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    n = weight.shape[2]
+    act = _activation("grouped_linear", activation)
+    odt = out.dtype if out is not None else out_dtype or x.dtype
+    _same_type("grouped_linear", x.dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
+    _same_type("grouped_linear", torch.int32, group_offsets=group_offsets, row_index=row_index)
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    w, layout = _matrix("grouped_linear", weight)
+    u = _matrix("grouped_linear", up_weight, layout)[0] if up_weight is not None else None
+    rows = x.shape[0] if row_index is None else row_index.shape[0]
+    if out is None:
+        out = torch.empty((rows, n), dtype=odt, device=x.device)
+    elif out.shape != (rows, n):
+        raise ValueError(f"grouped_linear: out has shape {tuple(out.shape)}, expected {(rows, n)}")
+    dev = x.device
+    _on(dev, _lib.load().sfb_grouped_linear, packed(x, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
+        packed(up_bias, "up_bias", dev), packed(group_offsets, "group_offsets", dev), packed(row_index, "row_index", dev), packed(out, "out", dev),
+        layout, dtype_code(x.dtype), dtype_code(odt), act, _status_ptr(status, dev))
+    return out
+
+
+class MoeRouting(NamedTuple):
+    """What :func:`moe_route` returns; assignment ``(t, j)`` is row ``positions[t, j]`` of the order sorted by expert."""
+
+    expert_ids: torch.Tensor  # int32 [T, top_k], -1 where a token has no candidate left
+    weights: torch.Tensor  # float32 [T, top_k]
+    group_offsets: torch.Tensor  # int32 [E + 1]: rows of expert e are group_offsets[e]:group_offsets[e + 1]
+    token_rows: torch.Tensor  # int32 [T * top_k]: the token of every row (grouped_linear's row_index), -1 behind the last
+    positions: torch.Tensor  # int32 [T, top_k], -1 where expert_ids is
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, workspace: torch.Tensor | None = None) -> MoeRouting:
+    """The ``top_k`` experts of every token (``logits [T, E]``; larger logit first, then lower index), their softmax weights
+    over the chosen experts (``renormalize``) or over all, and the assignments sorted by expert, then token.  A logit of
+    ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8,
+    :func:`moe_route_workspace_bytes`) is allocated when missing."""
+    if logits.dim() != 2:
+        raise ValueError(f"moe_route: logits [T, E], got {tuple(logits.shape)}")
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
+        logits = logits.contiguous()
+    (t, e), k, dev = logits.shape, int(top_k), logits.device
+    if k < 1 or k > min(e, 32):
+        raise ValueError(f"moe_route: top_k {k} outside 1 .. min(experts, 32)")
+    # one allocation for the five results
+    every = torch.empty(4 * t * k + e + 1, dtype=torch.int32, device=dev)
+    ids, weights, positions, rows, offsets = every.split([t * k] * 4 + [e + 1])
+    ids, weights, positions = ids.view(t, k), weights.view(torch.float32).view(t, k), positions.view(t, k)
+    need = moe_route_workspace_bytes(t, e)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace is not None and workspace.device != dev:
+        raise ValueError(f"moe_route: workspace on {workspace.device}, logits on {dev}")
+    _on(dev, _lib.load().sfb_moe_route, packed(logits, "logits", dev), packed(ids, "expert_ids", dev), packed(weights, "weights", dev),
+        packed(offsets, "group_offsets", dev), packed(rows, "token_rows", dev), packed(positions, "positions", dev), dtype_code(logits.dtype),
+        1 if renormalize else 0, workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0)
+    return MoeRouting(ids, weights, offsets, rows, positions)
+
+
+def moe_route_workspace_bytes(tokens: int, experts: int) -> int:
+    n = _lib.load().sfb_moe_route_workspace_bytes(int(tokens), int(experts))
+    if n < 0:
+        raise ValueError("invalid moe_route workspace query")
+    return int(n)
+
+
+def moe_combine(y: torch.Tensor, positions: torch.Tensor, weights: torch.Tensor, *, residual: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])``: every token's experts' rows (``y [R, H]``, the last
+    :func:`grouped_linear`'s result) back to the token; ``positions`` int32 and ``weights`` float32 ``[T, top_k]`` are
+    :func:`moe_route`'s.  A position of -1 adds nothing.  fp32 sums in the order of j, one rounding; ``out`` may be the residual."""
+    if y.dim() != 2 or positions.dim() != 2 or positions.shape != weights.shape:
+        raise ValueError(f"moe_combine: y [R, H], positions and weights [T, k], got {tuple(y.shape)}, {tuple(positions.shape)}, {tuple(weights.shape)}")
+    _same_type("moe_combine", torch.int32, positions=positions)
+    _same_type("moe_combine", torch.float32, weights=weights)
+    _same_type("moe_combine", y.dtype, residual=residual, out=out)
+    shape = (positions.shape[0], y.shape[1])
+    for name, t in (("out", out), ("residual", residual)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"moe_combine: {name} has shape {tuple(t.shape)}, expected {shape}")
+    if out is None:
+        out = torch.empty(shape, dtype=y.dtype, device=y.device)
+    dev = y.device
+    _on(dev, _lib.load().sfb_moe_combine, packed(y, "y", dev), packed(positions, "positions", dev), packed(weights, "weights", dev),
+        packed(residual, "residual", dev), packed(out, "out", dev), dtype_code(y.dtype), _status_ptr(status, dev))
+    return out

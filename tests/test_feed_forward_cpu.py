@@ -1,0 +1,98 @@
+"""Refusals of the feed-forward operators, without a GPU: every bad call ends in ValueError before a launch."""
+
+import pytest
+import torch
+
+from llm_compileforge_b200 import B200Backend, _lib, ops
+from test_abi_cpu import _fake_desc
+
+BF16 = torch.bfloat16
+
+
+def t(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.fused_linear(t(4, 8), t(16, 8)),  # K differs
+    lambda: ops.fused_linear(t(4, 8), t(8, 8, 2)),
+    lambda: ops.fused_linear(t(4, 0), t(0, 8)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8, dtype=torch.float16)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), t(8, dtype=torch.float32)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), activation="swish"),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), residual=t(4, 16)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), residual=t(4, 8, dtype=torch.float32)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), out=t(4, 4)),
+    lambda: ops.fused_linear(t(2, 4, 8), t(8, 8), out=t(4, 2, 8).transpose(0, 1)),
+    lambda: ops.fused_linear(t(4, 8), t(8, 8), up_weight=t(8, 8).t()[:, :], activation="silu"),
+    lambda: ops.fused_linear(t(4, 8), t(8, 32)[:, ::2]),
+    lambda: ops.grouped_linear(t(4, 8), t(8, 8), i32(2)),
+    lambda: ops.grouped_linear(t(4, 8), t(2, 8, 8), torch.zeros(3, dtype=torch.int64)),
+    lambda: ops.grouped_linear(t(4, 8), t(2, 8, 8), i32(3), row_index=torch.zeros(4)),
+    lambda: ops.grouped_linear(t(4, 8), t(2, 8, 8), i32(3), out=t(5, 8)),
+    lambda: ops.moe_route(t(4, 8), 9),
+    lambda: ops.moe_route(t(4, 8), 0),
+    lambda: ops.moe_route(t(4, 64), 33),
+    lambda: ops.moe_route(t(4, 8, 2), 1),
+    lambda: ops.moe_combine(t(4, 8), i32(2, 2), t(2, 2)),
+    lambda: ops.moe_combine(t(4, 8), i32(2, 2), torch.zeros(2, 3)),
+    lambda: ops.moe_combine(t(4, 8), torch.zeros(2, 2, dtype=torch.int64), torch.zeros(2, 2)),
+    lambda: ops.moe_combine(t(4, 8), i32(2, 2), torch.zeros(2, 2), residual=t(3, 8)),
+    # good calls, but on the CPU
+    lambda: ops.fused_linear(t(4, 8), t(8, 8)),
+    lambda: ops.moe_combine(t(4, 8), i32(2, 2), torch.zeros(2, 2)),
+])
+def test_bad_calls_raise_value_errors(call, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_names_of_the_executor():
+    assert {"fused_linear", "grouped_linear", "moe_route", "moe_combine"} <= set(B200Backend().supported_ops())
+
+
+def lin(x, w, b, u, ub, r, o, layout=0, dtype=1, odt=1, act=0):
+    import ctypes
+
+    p = lambda d: ctypes.cast(ctypes.pointer(d), ctypes.c_void_p) if d is not None else None  # noqa: E731
+    return _lib.load().sfb_fused_linear(p(x), p(w), p(b), p(u), p(ub), p(r), p(o), layout, dtype, odt, act, None, None)
+
+
+def test_library_refuses_bad_descriptors():
+    d = _fake_desc
+    x, w, o = d((4, 8), 2), d((8, 16), 2), d((4, 16), 2)
+    bad = [
+        (lin(x, d((16, 8), 2), None, None, None, None, o), "weight is"),
+        (lin(x, w, None, None, None, None, d((5, 16), 2)), "x [M, K]"),
+        (lin(x, w, d((8,), 2), None, None, None, o), "bias"),
+        (lin(x, w, None, None, d((16,), 2), None, o), "up_bias without"),
+        (lin(x, w, None, d((8, 8), 2), None, None, o), "up_weight must have"),
+        (lin(x, w, None, None, None, d((4, 8), 2), o), "residual"),
+        (lin(x, w, None, None, None, None, o, layout=2), "layout"),
+        (lin(x, w, None, None, None, None, o, act=9), "activation"),
+        (lin(x, w, None, None, None, None, o, dtype=3, odt=3), "fp32, bf16 or fp16"),
+        (lin(x, w, None, None, None, None, o, odt=2), "fp32, bf16 or fp16"),
+        (lin(x, w, None, None, None, None, d((4, 16), 2, strides=[8, 1])), "overlap"),
+        (lin(d((4, 8), 2, strides=[1, 4]), w, None, None, None, None, o), "contiguous"),
+        (lin(d((4, 0), 2), d((0, 16), 2), None, None, None, None, o), "K is zero"),
+        (lin(d((4, 8), 2, device=_lib.SFB_DEVICE_CPU), w, None, None, None, None, o), "CUDA"),
+        (lin(None, w, None, None, None, None, o), "NULL"),
+    ]
+    for rc, _ in bad:
+        assert rc in (_lib.SFB_ERR_INVALID_ARG, _lib.SFB_ERR_UNSUPPORTED)
+    for args, text in (((x, d((16, 8), 2), None, None, None, None, o), "weight is"), ((x, w, None, None, d((16,), 2), None, o), "up_bias without")):
+        lin(*args)
+        assert text in _lib.load().sfb_last_error().decode()
+    assert lin(d((0, 8), 2), w, None, None, None, None, d((0, 16), 2)) == _lib.SFB_OK  # nothing to do
+
+
+def test_route_workspace_query():
+    assert ops.moe_route_workspace_bytes(1, 64) == 0
+    assert ops.moe_route_workspace_bytes(128 * 3, 64) >= 3 * 64 * 4
+    with pytest.raises(ValueError):
+        ops.moe_route_workspace_bytes(-1, 4)
