@@ -480,8 +480,9 @@ SFB_API int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const 
  *   x [X, K]  weight, up_weight [E, K, N] or [E, N, K]  bias, up_bias [E, N] or NULL
  *   group_offsets int32 [E + 1], read on the device: not decreasing, within 0 .. R; groups may be empty
  *   row_index int32 [R] or NULL  out [R, N]
- * Rows of out outside every group are left as they were.  E <= 1024.  Offsets that leave 0 .. R are clamped, a
- * decreasing pair is an empty group, and a row index outside 0 .. X-1 reads row 0; each sets SFB_STATUS_BAD_ROW_INDEX. */
+ * Rows of out outside every group are left as they were.  E <= 1024.  Offsets that leave 0 .. R are clamped, one below
+ * an offset before it counts as that one, and a row index outside 0 .. X-1 reads row 0; each sets
+ * SFB_STATUS_BAD_ROW_INDEX. */
 SFB_API int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight,
                                const SFBTensor* up_bias, const SFBTensor* group_offsets, const SFBTensor* row_index, SFBTensor* out,
                                int weight_layout, int dtype, int out_dtype, int activation, int32_t* status, void* stream);

@@ -18,10 +18,19 @@ struct LinearArgs {
     int64_t w_stride[3], up_stride[3];         // group, k, n
     int64_t bias_stride, up_bias_stride;       // group
     int64_t rows, x_rows, K, N, groups;
-    int dtype, out_dtype, act;
+    int layout, dtype, out_dtype, act;
     int* status;
 };
 int launch_linear_generic(const LinearArgs& a, cudaStream_t stream);
+// Returns SFB_ERR_UNSUPPORTED (leaving the error text alone) for types and alignments outside what TMA and the tensor cores
+// take; the caller then runs the generic kernel.
+int launch_linear_tcgen05(const LinearArgs& a, cudaStream_t stream);
+struct LinearPlan {
+    int tokens;          // rows of out in a tile, at most
+    int split;           // thread blocks that share a tile's K steps
+    int64_t feat_tiles;  // tiles across the columns of out
+};
+LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, int sms);
 
 constexpr int kMaxGroups = 1024;  // groups (experts) of one call
 constexpr int kMaxTopK = 32;
@@ -54,13 +63,9 @@ struct CombineArgs {
 int launch_moe_combine(const CombineArgs& a, cudaStream_t stream);
 
 #ifdef __CUDACC__
-// Rows [begin, end) of group e.  Offsets come from the device and are not trusted: both ends are clamped to [0, rows]
-// and a pair that decreases is an empty group, so no address follows from a bad one.
-__device__ __forceinline__ int2 group_rows(const int32_t* offsets, int e, int rows) {
-    const int b = offsets[e], t = offsets[e + 1];
-    const int lo = min(max(b, 0), rows);
-    return make_int2(lo, max(lo, min(max(t, 0), rows)));
-}
+// Group offsets come from the device and are not trusted: each is clamped to [0, rows], and one below an offset before it
+// counts as that one.  Groups then never overlap or leave the rows, whatever the array holds.
+__device__ __forceinline__ int group_offset(int raw, int before, int rows) { return max(before, min(raw, rows)); }
 
 // The activations in fp32.  silu and the tanh form of gelu as h * logistic(.), the erf form as h/2 * erfc(-h / sqrt 2):
 // none of them subtracts nearly equal numbers for large negative h.

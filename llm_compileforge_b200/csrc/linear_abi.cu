@@ -64,12 +64,19 @@ int linear_views(const char* op, const SFBTensor* x, const SFBTensor* weight, co
     a->x_stride = vx.stride[2];
     a->out = vo.base;
     a->out_stride = vo.stride[2];
+    a->layout = layout;
     a->dtype = dtype;
     a->out_dtype = out_dtype;
     a->act = activation;
     const int64_t most = 0x7fffffffLL;
     if (a->rows > most || a->x_rows > most || a->K > most || a->N > most) return fail(SFB_ERR_UNSUPPORTED, "%s: dimension too large", op);
     return SFB_OK;
+}
+
+// The tensor cores where TMA can address the operands, else the CUDA cores.
+int launch_linear(const LinearArgs& a, cudaStream_t stream) {
+    const int rc = launch_linear_tcgen05(a, stream);
+    return rc == SFB_ERR_UNSUPPORTED ? launch_linear_generic(a, stream) : rc;
 }
 
 }  // namespace
@@ -93,7 +100,7 @@ int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTenso
     if (a.rows == 0 || a.N == 0) return SFB_OK;
     if (a.K == 0) return fail(SFB_ERR_INVALID_ARG, "fused_linear: K is zero");
     a.status = status;
-    return launch_linear_generic(a, static_cast<cudaStream_t>(stream));
+    return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
 
 int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight, const SFBTensor* up_bias,
@@ -119,7 +126,7 @@ int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTen
     if (a.rows == 0 || a.N == 0) return SFB_OK;
     if (a.K == 0) return fail(SFB_ERR_INVALID_ARG, "grouped_linear: K is zero");
     a.status = status;
-    return launch_linear_generic(a, static_cast<cudaStream_t>(stream));
+    return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
 
 int64_t sfb_moe_route_workspace_bytes(int64_t tokens, int64_t experts) {

@@ -24,22 +24,25 @@ __global__ void __launch_bounds__(256) linear_generic_kernel(const LinearArgs a)
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
 
     if (tid == 0) {  // row tile blockIdx.x -> its group: groups take ceil(rows / 64) tiles each, one after another
-        int left = (int)blockIdx.x, e = 0, lo = 0, hi = (int)a.rows;
+        int left = (int)blockIdx.x, e = 0, lo = 0, hi = (int)a.rows, flag = 0;
         bool found = !a.offsets && (int64_t)left * kTile < a.rows;
-        for (; a.offsets && e < a.groups && !found; ++e) {
-            const int2 r = group_rows(a.offsets, e, (int)a.rows);
-            lo = r.x; hi = r.y;
-            const int tiles = (hi - lo + kTile - 1) / kTile;
-            found = left < tiles;
-            if (found) break;
-            left -= tiles;
+        if (a.offsets) {
+            hi = group_offset(a.offsets[0], 0, (int)a.rows);
+            flag = hi != a.offsets[0];
+            for (; e < a.groups && !found; ++e) {
+                lo = hi;
+                hi = group_offset(a.offsets[e + 1], lo, (int)a.rows);
+                flag |= hi != a.offsets[e + 1];
+                const int tiles = (hi - lo + kTile - 1) / kTile;
+                found = left < tiles;
+                if (found) break;
+                left -= tiles;
+            }
+            if (flag && a.status) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
         }
         tile_of[0] = found ? e : -1;
         tile_of[1] = lo + left * kTile;
         tile_of[2] = hi;
-        if (a.offsets && a.status && blockIdx.x == 0 && blockIdx.y == 0)
-            for (int i = 0; i <= a.groups; ++i)
-                if (a.offsets[i] < (i ? a.offsets[i - 1] : 0) || a.offsets[i] > a.rows) { atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX); break; }
     }
     __syncthreads();
     const int e = tile_of[0], row0 = tile_of[1], row_end = tile_of[2];
@@ -115,8 +118,9 @@ __global__ void __launch_bounds__(256) linear_generic_kernel(const LinearArgs a)
 
 template <typename T, typename TO>
 int launch(const LinearArgs& a, cudaStream_t stream) {
-    // every group rounds its rows up to whole tiles: at most one tile more per group than the rows fill
-    const int64_t row_tiles = ceil_div(a.rows, (int64_t)kTile) + (a.offsets ? std::min(a.groups, a.rows) : 0);
+    // every group rounds its rows up to whole tiles: at most one tile more per group than the rows fill, and one that only
+    // reads the offsets to their end
+    const int64_t row_tiles = ceil_div(a.rows, (int64_t)kTile) + (a.offsets ? std::min(a.groups, a.rows) + 1 : 0);
     const int64_t col_tiles = ceil_div(a.N, (int64_t)kTile);
     if (row_tiles > 0x7fffffffLL || col_tiles > 65535) return fail(SFB_ERR_UNSUPPORTED, "linear: too many tiles");
     const dim3 grid((unsigned)row_tiles, (unsigned)col_tiles);
