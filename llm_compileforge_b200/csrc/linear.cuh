@@ -27,6 +27,7 @@ int launch_linear_generic(const LinearArgs& a, cudaStream_t stream);
 int launch_linear_tcgen05(const LinearArgs& a, cudaStream_t stream);
 struct LinearPlan {
     int tokens;          // rows of out in a tile, at most
+    int pair;            // 1: a cluster of two thread blocks on each tile (256 features)
     int split;           // thread blocks that share a tile's K steps
     int64_t feat_tiles;  // tiles across the columns of out
 };

@@ -9,12 +9,18 @@
 // thread block whatever the shape.
 //
 // Persistent thread blocks walk the tiles; accumulators are double-buffered in tensor memory (2 x kTok columns):
-//   warp 4    TMA producer: per 64-wide K step two boxes of 64 features, and the token rows as boxes of box_rows rows or, with a
-//             row index, four rows per gather load; one lane per box
-//   warp 5    one thread issues tcgen05.mma kind::f16 (M 128, N = tokens, K 16, four per step); the weight operand is
-//             MN-major for [K, N] storage and K-major for [N, K], straight from 128-byte-swizzled shared memory
-//   warps 0-3 epilogue: 16 tokens at a time through a transposing buffer in shared memory, so that rows of out and
-//             residual move as 8 bytes a lane; bias, activation, gate, residual in fp32, one rounding
+//   warp 8      TMA producer: per 64-wide K step two boxes of 64 features, and the token rows as boxes of box_rows rows
+//   warps 10-13 with a row index, the token rows instead: 16-byte cp.async pieces, placed as the 128-byte swizzle asks.  (TMA's
+//               own row gather takes four rows an instruction and about 60 clocks for each: 4000 clocks for a K step of 256
+//               rows whose MMAs take 512.)
+//   warp 9      one thread issues tcgen05.mma kind::f16 (N = tokens, K 16, four per step); the weight operand is MN-major for
+//               [K, N] storage and K-major for [N, K], straight from 128-byte-swizzled shared memory
+//   warps 0-7   epilogue, two groups of four warps that take every other 16 tokens: through a transposing buffer in shared
+//               memory, so that rows of out and residual move as 8 bytes a lane; bias, activation, gate, residual in fp32,
+//               one rounding
+// Many rows a group (kPair): a cluster of two thread blocks owns 256 features x 256 tokens with cta_group::2 MMAs (M 256): each
+// block loads its 128 features and half of the tokens, the leader's MMAs read both, each block's tensor memory receives its
+// own features.
 // Few tiles (decode): a cluster of up to eight thread blocks shares a tile, each taking a part of K; the parts meet in the
 // epilogue through distributed shared memory, summed in the order of the ranks - no workspace, no atomics, the same bits
 // every time.
@@ -24,8 +30,10 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "linear.cuh"
 
@@ -35,8 +43,10 @@ namespace {
 constexpr int kFeat = 128, kStepK = 64, kChunk = 16;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
-constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]
-constexpr int kThreads = 192;
+constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]; two for each epilogue group
+constexpr int kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 10, kGatherThreads = 128;
+constexpr int kThreads = 32 * kGatherWarp;       // without a row index
+constexpr int kGatherLag = 3;                    // K steps of gathered rows in flight behind the one being issued
 constexpr uint32_t kSpin = 1u << 21;
 constexpr int kMaxSplit = 8;
 
@@ -46,26 +56,40 @@ enum {
     B_EMPTY = kMaxStages,
     B_ACC_FULL = 2 * kMaxStages,
     B_ACC_EMPTY = B_ACC_FULL + 2,
-    B_PART_FULL = B_ACC_EMPTY + 2,   // a chunk's partial sums lie in every block's staging buffer
-    B_PART_EMPTY = B_PART_FULL + 2,  // every block has read the chunk
-    B_COUNT = B_PART_EMPTY + 2
+    B_PART_FULL = B_ACC_EMPTY + 2,   // per epilogue group and buffer: a chunk's partial sums lie in every block's buffer
+    B_PART_EMPTY = B_PART_FULL + 4,  // every block has read the chunk
+    B_COUNT = B_PART_EMPTY + 4
 };
 
-constexpr int stage_bytes(int tok) { return kWBytes + tok * 128; }
-constexpr int smem_bytes(int tok, int stages, int groups) {
-    return 1024 + stages * stage_bytes(tok) + 2 * kStaging + B_COUNT * 8 + 16 + (3 * groups + 1) * 4;
-}
+// A kernel's shape: token columns of a tile, pipeline stages, whether a cluster of two shares each tile.
+template <int TOK, int STAGES, bool PAIR>
+struct Shape {
+    static constexpr int kTok = TOK, kStages = STAGES;
+    static constexpr bool kPair = PAIR;
+    static constexpr int kRows = PAIR ? TOK / 2 : TOK;  // token rows in one block's shared memory
+    static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
+    static constexpr int kStage = kWBytes + kRows * 128;
+    static constexpr int smem(int groups) { return 1024 + kStages * kStage + 4 * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
+    static_assert(STAGES <= kMaxStages && STAGES > kGatherLag + 1, "pipeline depth");
+};
+// About 160 KB of operands in flight whatever the width
+using Shape32 = Shape<32, 8, false>;
+using Shape64 = Shape<64, 7, false>;
+using Shape128 = Shape<128, 5, false>;
+using ShapePair = Shape<256, 5, true>;
+static_assert(Shape32::smem(kMaxGroups) <= 232448 && Shape64::smem(kMaxGroups) <= 232448 && Shape128::smem(kMaxGroups) <= 232448 &&
+              ShapePair::smem(kMaxGroups) <= 232448, "shared memory of one thread block");
 
 struct TileArgs {
-    const void *bias, *up_bias, *residual;
+    const void *x, *bias, *up_bias, *residual;
     void* out;
     const int32_t *offsets, *row_index;
     int* status;
-    int64_t out_stride, res_stride, bias_stride, up_bias_stride;
-    int rows, x_rows, N, n_k, groups;
+    int64_t x_stride, out_stride, res_stride, bias_stride, up_bias_stride;
+    int rows, x_rows, N, K, n_k, groups;
     int feat_tiles;  // column tiles of out
     int box_rows;    // token rows of one TMA box
-    int split;       // thread blocks that share a tile's K steps (= cluster size)
+    int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair)
     int block;       // token tiles that run together through the feature tiles (L2 reuse of x and W)
     int act;
     bool gated, nk, out_f32, vec;
@@ -136,41 +160,69 @@ __device__ __forceinline__ void ld_shared(float* v, uint32_t addr) {
         else asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory");
     }
 }
+template <bool PAIR>  // PAIR: the bytes are reported to a barrier of the cluster's leader
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
-// Four rows of a map whose box is one row high, side by side at dst.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int4 r) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                 ::"r"(dst), "l"(map), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
-                 : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // bytes < 16: the rest is zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
 }
+template <bool PAIR>
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <bool PAIR>  // PAIR: arrives on this barrier in both thread blocks
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                        uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n}\n"
-        ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n}\n"
+            ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n}\n"
+            ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -203,17 +255,26 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
     if constexpr (BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
     else return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-// Whether any of the four epilogue warps failed; all of them come here, so none waits for one that has left.
-__device__ __forceinline__ bool epilogue_any(bool failed) {
+// Whether any of an epilogue group's four warps failed; all of them come here, so none waits for one that has left.
+__device__ __forceinline__ bool group_any(int barrier, bool failed) {
     uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
                  : "=r"(r)
-                 : "r"((uint32_t)failed)
+                 : "r"((uint32_t)failed), "r"(barrier)
                  : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void epilogue_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void group_sync(int barrier) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(barrier) : "memory"); }
 
+// h Phi(h).  erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + p z), for z >= 0: Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26, absolute error 1.5e-7 - a quarter of the instructions of erfcf, which made the epilogue of
+// a [1001, 2048] x [2048, 8192] product take four times its MMAs.
+__device__ __forceinline__ float gelu_erf(float h) {
+    const float z = fabsf(h) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float q = 0.5f * poly * __expf(-z * z);  // Phi(-|h|)
+    return h * (h < 0.f ? q : 1.f - q);
+}
 template <int W>
 __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
     auto each = [&](auto f) {
@@ -221,7 +282,7 @@ __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
         for (int i = 0; i < W; ++i) h[i] = f(h[i]);
     };
     if (act == SFB_ACT_SILU) each([](float v) { return __fdividef(v, 1.f + __expf(-v)); });
-    else if (act == SFB_ACT_GELU) each([](float v) { return activate<SFB_ACT_GELU>(v); });
+    else if (act == SFB_ACT_GELU) each([](float v) { return gelu_erf(v); });
     else if (act == SFB_ACT_GELU_TANH) each([](float v) { return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v))); });
     else if (act == SFB_ACT_RELU) each([](float v) { return activate<SFB_ACT_RELU>(v); });
 }
@@ -229,69 +290,74 @@ __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
 struct Tile {
     int group, row0, rows, feat;
 };
-// The groups of a call in shared memory: first row, number of rows, and token tiles before each group.
+// The groups of a call in shared memory: group e has rows off[e] .. off[e + 1], and tiles[e] token tiles lie before it.
 struct Groups {
-    const int *lo, *count, *tiles;
+    const int *off, *tiles;
     int n;
     // Tile t: groups one after another; inside a group blocks of `block` token tiles, token tiles fastest, then features.  A
-    // group's rows are spread evenly over its token tiles, in sixteens.
-    __device__ __forceinline__ Tile at(int t, int tok, int feat_tiles, int block) const {
+    // group's rows are spread evenly over its token tiles, in multiples of `round`.
+    __device__ __forceinline__ Tile at(int t, int feat_tiles, int block, int round) const {
         int e = 0;
-        for (int step = 512; step > 0; step >>= 1)
+        for (int step = kMaxGroups / 2; step > 0; step >>= 1)
             if (e + step < n && tiles[e + step] * feat_tiles <= t) e += step;
-        const int nt = tiles[e + 1] - tiles[e];
+        const int nt = tiles[e + 1] - tiles[e], count = off[e + 1] - off[e];
         int i = t - tiles[e] * feat_tiles;
         const int b = i / (block * feat_tiles);
         const int g = min(block, nt - b * block);
         i -= b * block * feat_tiles;
         const int f = i / g, m = b * block + i - f * g;
-        const int per = token_rows(count[e], nt);
-        return {e, lo[e] + m * per, min(per, count[e] - m * per), f};
+        const int per = ((count + nt - 1) / nt + round - 1) / round * round;
+        return {e, off[e] + m * per, min(per, count - m * per), f};
     }
-    static __device__ __forceinline__ int token_rows(int count, int nt) { return (((count + nt - 1) / nt) + 15) & ~15; }
 };
 
-template <int kTok, int kStages, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename S, bool BF16>
+__global__ void __launch_bounds__(kThreads + kGatherThreads, 1)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                       const TileArgs a) {
     extern __shared__ uint8_t smem_raw[];
-    static_assert(kStages <= kMaxStages, "barrier slots");
-    constexpr int kStage = stage_bytes(kTok);
+    constexpr int kTok = S::kTok, kStages = S::kStages, kStage = S::kStage;
+    constexpr bool PAIR = S::kPair;
+    using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = a.split;
-    const int rank = split > 1 ? (int)cluster_rank() : 0;
-    const int unit = (int)blockIdx.x / split, n_units = (int)gridDim.x / split;
+    const int split = PAIR ? 1 : a.split, cluster = PAIR ? 2 : split;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+    const int unit = (int)blockIdx.x / cluster, n_units = (int)gridDim.x / cluster;
+    const bool gather = a.row_index != nullptr;
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
     float* staging = reinterpret_cast<float*>(base_ptr + kStages * kStage);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + 2 * kStaging);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + 4 * kStaging);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
-    int* g_lo = reinterpret_cast<int*>(tmem_slot + 4);
-    int* g_count = g_lo + a.groups;
-    int* g_tiles = g_count + a.groups;
+    int* g_off = reinterpret_cast<int*>(tmem_slot + 4);
+    int* g_tiles = g_off + a.groups + 1;
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+    auto leader_bar = [&](int i) { return PAIR ? peer_addr(bar(i), 0) : bar(i); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(bar(B_FULL + s), 1);
+            // the TMA producer's arrive with the bytes, and the gathering warps (of both blocks, on the leader's barrier)
+            mbar_init(bar(B_FULL + s), 1 + (gather ? kGatherThreads / 32 * (PAIR ? 2 : 1) : 0));
             mbar_init(bar(B_EMPTY + s), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_ACC_FULL + i), 1);
-            mbar_init(bar(B_ACC_EMPTY + i), 4);
+            mbar_init(bar(B_ACC_EMPTY + i), kEpilogueWarps * (PAIR ? 2 : 1));
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(bar(B_PART_FULL + i), 4 * split);
             mbar_init(bar(B_PART_EMPTY + i), 4 * split);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 5) tmem_alloc(smem_u32(tmem_slot), 2 * kTok);
+    if (warp == kMmaWarp) tmem_alloc<PAIR>(smem_u32(tmem_slot), 2 * kTok);
     if (warp == 0) {  // the groups' rows, and the running number of token tiles
         int before = 0, top = a.offsets ? group_offset(a.offsets[0], 0, a.rows) : 0;
         bool bad = a.offsets && top != a.offsets[0];
+        if (lane == 0) g_off[0] = top;
         for (int e0 = 0; e0 < a.groups; e0 += 32) {
             const int e = e0 + lane;
             const int raw = a.offsets && e < a.groups ? a.offsets[e + 1] : a.rows;
@@ -312,7 +378,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 const int up = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += up;
             }
-            if (e < a.groups) { g_lo[e] = lo; g_count[e] = hi - lo; g_tiles[e] = before + sum - own; }
+            if (e < a.groups) { g_off[e + 1] = hi; g_tiles[e] = before + sum - own; }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (lane == 0) g_tiles[a.groups] = before;
@@ -320,65 +386,101 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (split > 1) cluster_sync();  // the other blocks' barriers exist before anything is sent to them
+    if (cluster > 1) cluster_sync();  // the other blocks' barriers exist before anything is sent to them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const Groups groups{g_lo, g_count, g_tiles, a.groups};
+    const Groups groups{g_off, g_tiles, a.groups};
     const int tiles_total = g_tiles[a.groups] * a.feat_tiles;
-    const int k_first = (int)((int64_t)a.n_k * rank / split), k_end = (int)((int64_t)a.n_k * (rank + 1) / split);
-    const int feats = a.gated ? kFeat / 2 : kFeat;  // columns of out in a tile
+    const int k_first = PAIR ? 0 : (int)((int64_t)a.n_k * rank / split), k_end = PAIR ? a.n_k : (int)((int64_t)a.n_k * (rank + 1) / split);
+    const int feats = a.gated ? kFeat / 2 : kFeat;  // columns of out that this thread block computes of a tile
+    // first such column of a tile; and of a tile's tokens (PAIR: the MMA takes half of its N from each block) the ones whose
+    // rows of x this block brings in
+    auto column0 = [&](const Tile& t) { return (PAIR ? 2 * t.feat + rank : t.feat) * feats; };
+    auto half_of = [&](const Tile& t) { return PAIR ? (t.rows + 31) / 32 * 16 : t.rows; };
+    auto own_rows = [&](const Tile& t, int r) { return PAIR ? max(0, min(half_of(t), t.rows - r * half_of(t))) : t.rows; };
     bool timed_out = false;
 
-    if (warp == 4) {
+    if (warp == kTmaWarp) {
         // ============================ TMA producer ============================
-        // Lanes 0 and 1 load the weights; without a row index lane 2 + j loads token box j, with one every lane the rows of
-        // its quads of tokens.
+        // Lanes 0 and 1 load the weights, lane 2 + j token box j.
         uint32_t s = 0, ephase = 1;
         for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
-            const Tile tile = groups.at(t, kTok, a.feat_tiles, a.block);
-            const int n0 = tile.feat * feats + (a.gated ? 0 : lane * 64);  // lanes 0 and 1
+            const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+            const int n0 = column0(tile) + (a.gated ? 0 : lane * 64);  // lanes 0 and 1
             const CUtensorMap* my_w = a.gated && lane == 1 ? &umap : &wmap;
-            const int boxes = a.row_index ? (tile.rows + 3) / 4 : (tile.rows + a.box_rows - 1) / a.box_rows;
-            const uint32_t bytes = kWBytes + boxes * (a.row_index ? 4 : a.box_rows) * 128;
-            int4 quad[kTok / 128 > 0 ? (kTok + 127) / 128 : 1];
-            constexpr int kQuads = sizeof(quad) / sizeof(quad[0]);
-            if (a.row_index) {
-#pragma unroll
-                for (int q = 0; q < kQuads; ++q) {
-                    int r[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int m = 4 * (lane + 32 * q) + i;
-                        r[i] = m < tile.rows ? a.row_index[tile.row0 + m] : 0;
-                        if (r[i] < 0 || r[i] >= a.x_rows) {
-                            if (a.status) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
-                            r[i] = 0;
-                        }
-                    }
-                    quad[q] = make_int4(r[0], r[1], r[2], r[3]);
-                }
-            }
+            auto boxes_of = [&](int r) { return gather ? 0 : (own_rows(tile, r) + a.box_rows - 1) / a.box_rows; };
+            const int boxes = boxes_of(rank), all = PAIR ? boxes_of(0) + boxes_of(1) : boxes;
+            const uint32_t bytes = (PAIR ? 2 : 1) * kWBytes + all * a.box_rows * 128;
+            const int row0 = tile.row0 + (PAIR ? rank * half_of(tile) : 0);
             for (int k = k_first; k < k_end; ++k) {
-                if (!mbar_wait(bar0 + 8u * (B_EMPTY + s), ephase)) { timed_out = true; break; }
-                const uint32_t full = bar0 + 8u * (B_FULL + s), dst = base + s * kStage;
-                if (lane == 0) mbar_expect_tx(full, bytes);
+                if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
+                const uint32_t dst = base + s * kStage;
+                if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), bytes);
                 __syncwarp();
+                const uint32_t full = leader_bar(B_FULL + s);
                 const int k0 = k * kStepK;
-                if (lane < 2) tma_load_3d(dst + lane * kHalfBytes, my_w, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
-                if (a.row_index) {
-#pragma unroll
-                    for (int q = 0; q < kQuads; ++q)
-                        if (lane + 32 * q < boxes) tma_gather4(dst + kWBytes + (lane + 32 * q) * 512, &xmap, full, k0, quad[q]);
-                } else if (lane >= 2 && lane - 2 < boxes) {
-                    tma_load_2d(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, tile.row0 + (lane - 2) * a.box_rows);
-                }
+                if (lane < 2) tma_load_3d<PAIR>(dst + lane * kHalfBytes, my_w, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
+                else if (lane - 2 < boxes) tma_load_2d<PAIR>(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, row0 + (lane - 2) * a.box_rows);
                 if (++s == kStages) { s = 0; ephase ^= 1; }
             }
         }
         timed_out = __any_sync(0xffffffffu, timed_out);
-    } else if (warp == 5) {
+    } else if (warp >= kGatherWarp) {
+        // ====================== rows of x by their index ======================
+        // Thread i copies 16-byte piece i & 7 of rows i / 8, i / 8 + 16, ...  A K step is announced kGatherLag steps after it was
+        // issued: by then its copies are usually done.  The copies are the generic proxy's and the MMA reads through the async
+        // one, so each thread fences its own before its warp arrives.
+        constexpr int kEach = S::kRows / 16;
+        const int i = threadIdx.x - kThreads, piece = i & 7;
+        uint32_t s = 0, ephase = 1, announced = 0;  // announced: stage of the next K step to announce
+        int behind = 0;                             // steps issued and not announced
+        auto announce = [&] {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(leader_bar(B_FULL + announced));
+                else mbar_arrive(bar(B_FULL + announced));
+            }
+            if (++announced == kStages) announced = 0;
+            --behind;
+        };
+        for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
+            const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+            const int rows = own_rows(tile, rank), row0 = tile.row0 + (PAIR ? rank * half_of(tile) : 0);
+            const T* src[kEach];
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int m = i / 8 + 16 * j;
+                int r = m < rows ? a.row_index[row0 + m] : 0;
+                if (r < 0 || r >= a.x_rows) {
+                    if (a.status) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
+                    r = 0;
+                }
+                src[j] = static_cast<const T*>(a.x) + (int64_t)r * a.x_stride;
+            }
+            for (int k = k_first; k < k_end; ++k) {
+                if (__any_sync(0xffffffffu, !mbar_wait(bar(B_EMPTY + s), ephase))) { timed_out = true; break; }
+                const int k0 = k * kStepK + piece * 8;
+                const int bytes = max(0, min(16, (a.K - k0) * 2));
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    const int m = i / 8 + 16 * j;
+                    if (m < rows) cp_async16(base + s * kStage + kWBytes + m * 128 + ((piece ^ (m & 7)) << 4), src[j] + (bytes ? k0 : 0), bytes);
+                }
+                cp_async_commit();
+                ++behind;
+                if (behind > kGatherLag) {
+                    cp_async_wait<kGatherLag>();
+                    announce();
+                }
+                if (++s == kStages) { s = 0; ephase ^= 1; }
+            }
+        }
+        cp_async_wait<0>();
+        while (behind > 0) announce();
+    } else if (warp == kMmaWarp) {
         // ============================ MMA issuer ==============================
-        if (lane == 0) {
+        if (lane == 0 && (!PAIR || rank == 0)) {
             // [K, N] weights: rows of k, blocks of 64 features 8 KB apart, 16 k further = 2 KB; [N, K]: rows of features, 16 k
             // further = 32 bytes inside the swizzled row
             const uint32_t w_lo0 = desc_lo(base, a.nk ? 16 : kHalfBytes), x_lo0 = desc_lo(base + kWBytes, 16), hi = desc_hi(1024);
@@ -387,124 +489,72 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             uint32_t s = 0, phase = 0, off = 0;
             int it = 0;
             for (int t = unit; t < tiles_total && ok; t += n_units, ++it) {
-                const Tile tile = groups.at(t, kTok, a.feat_tiles, a.block);
-                const uint32_t idesc = instr_desc(BF16, !a.nk, kFeat, (tile.rows + 15) & ~15);
+                const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+                const uint32_t idesc = instr_desc(BF16, !a.nk, PAIR ? 2 * kFeat : kFeat, (tile.rows + S::kRound - 1) / S::kRound * S::kRound);
                 const int buf = it & 1;
                 ok = mbar_wait(bar(B_ACC_EMPTY + buf), ((it >> 1) & 1) ^ 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * kTok;
                 for (int k = k_first; k < k_end; ++k) {
-                    ok = mbar_wait(bar0 + 8u * (B_FULL + s), phase);
+                    ok = PAIR ? mbar_wait_cluster(bar(B_FULL + s), phase) : mbar_wait(bar(B_FULL + s), phase);
                     if (!ok) break;
                     tc_fence_after();
-                    mma_ss(d, w_lo0 + off, hi, x_lo0 + off, hi, idesc, k > k_first);
-                    mma_ss(d, w_lo0 + off + w_step, hi, x_lo0 + off + 2, hi, idesc, 1);
-                    mma_ss(d, w_lo0 + off + 2 * w_step, hi, x_lo0 + off + 4, hi, idesc, 1);
-                    mma_ss(d, w_lo0 + off + 3 * w_step, hi, x_lo0 + off + 6, hi, idesc, 1);
-                    tc_commit(bar0 + 8u * (B_EMPTY + s));
+                    mma_ss<PAIR>(d, w_lo0 + off, hi, x_lo0 + off, hi, idesc, k > k_first);
+                    mma_ss<PAIR>(d, w_lo0 + off + w_step, hi, x_lo0 + off + 2, hi, idesc, 1);
+                    mma_ss<PAIR>(d, w_lo0 + off + 2 * w_step, hi, x_lo0 + off + 4, hi, idesc, 1);
+                    mma_ss<PAIR>(d, w_lo0 + off + 3 * w_step, hi, x_lo0 + off + 6, hi, idesc, 1);
+                    tc_commit<PAIR>(bar(B_EMPTY + s));
                     ++s;
                     off += kStage >> 4;
                     if (s == kStages) { s = 0; off = 0; phase ^= 1; }
                 }
-                if (ok) tc_commit(bar(B_ACC_FULL + buf));
+                if (ok) tc_commit<PAIR>(bar(B_ACC_FULL + buf));
             }
             timed_out = !ok;
         }
     } else {
         // ============================== epilogue ==============================
-        using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+        const int group = warp >> 2, w4 = warp & 3;  // this group takes chunks group, group + 2, ..
+        const int sync_id = 1 + group;
         bool ok = true;
-        int it = 0, chunk = 0;
+        int it = 0, used = 0;  // chunks that this group has staged
         const int cols = a.gated ? 2 : 4;  // columns of out that a lane writes for a token
+        // vec: lane l holds columns cols * l ..; else l, l + 32, ..
+        const int col0 = a.vec ? cols * lane : lane, col_step = a.vec ? 1 : 32;
         for (int t = unit; t < tiles_total; t += n_units, ++it) {
-            const Tile tile = groups.at(t, kTok, a.feat_tiles, a.block);
-            const int buf = it & 1, n0 = tile.feat * feats;
-            // vec: lane l holds columns cols * l ..; else l, l + 32, ..
-            const int col0 = a.vec ? cols * lane : lane, col_step = a.vec ? 1 : 32;
-            float bias[4] = {}, up_bias[4] = {};
+            const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+            const int buf = it & 1, n = column0(tile) + col0;
+            float bias[4] = {}, up_bias[2] = {};
             const T* bp = a.bias ? static_cast<const T*>(a.bias) + tile.group * a.bias_stride : nullptr;
             const T* cp = a.up_bias ? static_cast<const T*>(a.up_bias) + tile.group * a.up_bias_stride : nullptr;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int n = n0 + col0 + i * col_step;
-                if (i < cols && n < a.N) {
-                    if (bp) bias[i] = to_float(bp[n]);
-                    if (cp) up_bias[i] = to_float(cp[n]);
+                const int c = n + i * col_step;
+                if (i < cols && c < a.N) {
+                    if (bp) bias[i] = to_float(bp[c]);
+                    if (cp && i < 2) up_bias[i] = to_float(cp[c]);
                 }
             }
-            if (ok) ok = mbar_wait(bar(B_ACC_FULL + buf), (it >> 1) & 1);
-            if (epilogue_any(!ok)) { ok = false; break; }
+            if (ok) ok = PAIR ? mbar_wait_cluster(bar(B_ACC_FULL + buf), (it >> 1) & 1) : mbar_wait(bar(B_ACC_FULL + buf), (it >> 1) & 1);
+            if (group_any(sync_id, !ok)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(warp * 32) << 16) + buf * kTok;
+            const uint32_t acc = tmem + ((uint32_t)(w4 * 32) << 16) + buf * kTok;
             const int chunks = (tile.rows + kChunk - 1) / kChunk;
-
-            // one token's row out of `sums` (four staged values of this lane): bias, activation, gate, residual, store
-            auto finish = [&](int m, float4 sums) {
-                const int64_t row = tile.row0 + m;
-                float h[4] = {sums.x, sums.y, sums.z, sums.w}, v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] += i < cols ? bias[i] : up_bias[i - 2];
-                if (a.gated) {
-                    float g[2] = {h[0], h[1]};
-                    activate_all(g, a.act);
-                    v[0] = g[0] * h[2]; v[1] = g[1] * h[3]; v[2] = v[3] = 0.f;
-                } else {
-                    activate_all(h, a.act);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = h[i];
-                }
-                const int n = n0 + col0;
-                if (a.vec) {
-                    if (n >= a.N) return;  // N is a multiple of cols
-                    if (a.out_f32) {
-                        float* o = static_cast<float*>(a.out) + row * a.out_stride + n;
-                        const float* r = static_cast<const float*>(a.residual) + row * a.res_stride + n;
-                        if (a.gated) {
-                            float2 q = a.residual ? *reinterpret_cast<const float2*>(r) : make_float2(0.f, 0.f);
-                            *reinterpret_cast<float2*>(o) = make_float2(v[0] + q.x, v[1] + q.y);
-                        } else {
-                            float4 q = a.residual ? *reinterpret_cast<const float4*>(r) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            *reinterpret_cast<float4*>(o) = make_float4(v[0] + q.x, v[1] + q.y, v[2] + q.z, v[3] + q.w);
-                        }
-                        return;
-                    }
-                    T* o = static_cast<T*>(a.out) + row * a.out_stride + n;
-                    const T* r = static_cast<const T*>(a.residual) + row * a.res_stride + n;
-                    if (a.gated) {
-                        if (a.residual) {
-                            const float2 q = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(r));
-                            v[0] += q.x; v[1] += q.y;
-                        }
-                        *reinterpret_cast<uint32_t*>(o) = pack2<BF16>(v[0], v[1]);
-                    } else {
-                        if (a.residual) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(r);
-                            const float2 q = unpack2<BF16>(u.x), p = unpack2<BF16>(u.y);
-                            v[0] += q.x; v[1] += q.y; v[2] += p.x; v[3] += p.y;
-                        }
-                        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
-                    }
-                    return;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = n + 32 * i;
-                    if (i >= cols || c >= a.N) continue;
-                    if (a.out_f32) {
-                        const float q = a.residual ? static_cast<const float*>(a.residual)[row * a.res_stride + c] : 0.f;
-                        static_cast<float*>(a.out)[row * a.out_stride + c] = v[i] + q;
-                    } else {
-                        const float q = a.residual ? to_float(static_cast<const T*>(a.residual)[row * a.res_stride + c]) : 0.f;
-                        static_cast<T*>(a.out)[row * a.out_stride + c] = from_float<T>(v[i] + q);
-                    }
+            auto release = [&] {  // the accumulator goes back: the next-but-one tile may overwrite it
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_cluster(leader_bar(B_ACC_EMPTY + buf));
+                    else mbar_arrive(bar(B_ACC_EMPTY + buf));
                 }
             };
+            if (group >= chunks) release();
+
             // a token's staged sums for this lane, from the row at `addr` (of any block): its columns; with a gate those of the
             // gate, then those of the up projection
-            auto staged = [&](uint32_t addr, auto peer) {
+            auto staged = [&](uint32_t addr, auto peer, float (&q)[4]) {
                 constexpr bool P = decltype(peer)::value;
-                float q[4];
                 if (!a.vec) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) ld_shared<1, P>(q + i, addr + 4u * (uint32_t)(lane + 32 * i));
@@ -514,62 +564,143 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 } else {
                     ld_shared<4, P>(q, addr + 16u * (uint32_t)lane);
                 }
-                return make_float4(q[0], q[1], q[2], q[3]);
+            };
+            // the residual of one token's columns, and their place in out
+            auto residual_of = [&](int64_t row, float (&r)[4]) {
+                if (a.out_f32) {
+                    const float* p = static_cast<const float*>(a.residual) + row * a.res_stride + n;
+                    if (!a.vec) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i < cols && n + 32 * i < a.N) r[i] = p[32 * i];
+                    } else if (n < a.N) {
+                        if (a.gated) { const float2 v = *reinterpret_cast<const float2*>(p); r[0] = v.x; r[1] = v.y; }
+                        else { const float4 v = *reinterpret_cast<const float4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+                    }
+                    return;
+                }
+                const T* p = static_cast<const T*>(a.residual) + row * a.res_stride + n;
+                if (!a.vec) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < cols && n + 32 * i < a.N) r[i] = to_float(p[32 * i]);
+                } else if (n < a.N) {
+                    const uint2 u = a.gated ? make_uint2(*reinterpret_cast<const uint32_t*>(p), 0u) : *reinterpret_cast<const uint2*>(p);
+                    const float2 lo = unpack2<BF16>(u.x), hi = unpack2<BF16>(u.y);
+                    r[0] = lo.x; r[1] = lo.y; r[2] = hi.x; r[3] = hi.y;
+                }
+            };
+            auto store = [&](int64_t row, const float (&v)[4]) {
+                if (a.out_f32) {
+                    float* o = static_cast<float*>(a.out) + row * a.out_stride + n;
+                    if (!a.vec) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i < cols && n + 32 * i < a.N) o[32 * i] = v[i];
+                    } else if (n < a.N) {  // N is a multiple of cols
+                        if (a.gated) *reinterpret_cast<float2*>(o) = make_float2(v[0], v[1]);
+                        else *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                    return;
+                }
+                T* o = static_cast<T*>(a.out) + row * a.out_stride + n;
+                if (!a.vec) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < cols && n + 32 * i < a.N) o[32 * i] = from_float<T>(v[i]);
+                } else if (n < a.N) {
+                    if (a.gated) *reinterpret_cast<uint32_t*>(o) = pack2<BF16>(v[0], v[1]);
+                    else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
+                }
+            };
+            // COUNT tokens' sums -> bias, activation, gate
+            auto finish = [&](auto& q) {
+                constexpr int COUNT = sizeof(q) / sizeof(q[0]);
+                if (a.gated) {
+                    float g[2 * COUNT];
+#pragma unroll
+                    for (int j = 0; j < COUNT; ++j) { g[2 * j] = q[j][0] + bias[0]; g[2 * j + 1] = q[j][1] + bias[1]; }
+                    activate_all(g, a.act);
+#pragma unroll
+                    for (int j = 0; j < COUNT; ++j) { q[j][0] = g[2 * j] * (q[j][2] + up_bias[0]); q[j][1] = g[2 * j + 1] * (q[j][3] + up_bias[1]); }
+                } else {
+                    float h[4 * COUNT];
+#pragma unroll
+                    for (int j = 0; j < 4 * COUNT; ++j) h[j] = q[j / 4][j % 4] + bias[j % 4];
+                    activate_all(h, a.act);
+#pragma unroll
+                    for (int j = 0; j < 4 * COUNT; ++j) q[j / 4][j % 4] = h[j];
+                }
             };
 
-            for (int c = 0; c < chunks; ++c, ++chunk) {
+            for (int c = group; c < chunks; c += 2, ++used) {
                 float v[kChunk];
                 tmem_ld16(acc + c * kChunk, v);
-                if (c == chunks - 1) {  // the accumulator goes back: the next-but-one tile may overwrite it
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(B_ACC_EMPTY + buf));
-                }
-                const int b = chunk & 1, left = tile.rows - c * kChunk;
-                float* stage = staging + b * (kStaging / 4);
+                if (c + 2 >= chunks) release();
+                const int b = used & 1, left = tile.rows - c * kChunk;
+                const int64_t row0 = tile.row0 + c * kChunk;
+                float* stage = staging + (2 * group + b) * (kStaging / 4);
                 if (split == 1) {
+                    constexpr int kEach = kChunk / 4;
+                    float q[kEach][4], r[kEach][4];
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i) stage[i * kFeat + warp * 32 + lane] = v[i];
-                    epilogue_sync();  // one barrier a chunk: a buffer is written again two chunks on, after the next chunk's barrier
+                    for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                    if (a.residual) {
 #pragma unroll
-                    for (int i = 0; i < kChunk / 4; ++i) {
-                        const int m = warp + 4 * i;
-                        if (m < left) finish(c * kChunk + m, staged(smem_u32(stage + m * kFeat), std::false_type{}));
+                        for (int i = 0; i < kEach; ++i)
+                            if (w4 + 4 * i < left) residual_of(row0 + w4 + 4 * i, r[i]);
                     }
+                    group_sync(sync_id);  // one barrier a chunk: a buffer is written again two chunks on, after the next chunk's barrier
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) staged(smem_u32(stage + (w4 + 4 * i) * kFeat), std::false_type{}, q[i]);
+                    finish(q);
+                    if (a.residual) {
+#pragma unroll
+                        for (int i = 0; i < 4 * kEach; ++i) q[i / 4][i % 4] += r[i / 4][i % 4];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i)
+                        if (w4 + 4 * i < left) store(row0 + w4 + 4 * i, q[i]);
                 } else {
-                    ok = ok && mbar_wait_cluster(bar(B_PART_EMPTY + b), ((chunk >> 1) & 1) ^ 1);
+                    ok = ok && mbar_wait_cluster(bar(B_PART_EMPTY + 2 * group + b), ((used >> 1) & 1) ^ 1);
                     if (!ok) break;
 #pragma unroll
                     for (int i = 0; i < kChunk; ++i)
-                        if (i < left) stage[i * kFeat + warp * 32 + lane] = v[i];
+                        if (i < left) stage[i * kFeat + w4 * 32 + lane] = v[i];
                     __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_FULL + b), lane));
-                    ok = mbar_wait_cluster(bar(B_PART_FULL + b), (chunk >> 1) & 1);
+                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_FULL + 2 * group + b), lane));
+                    ok = mbar_wait_cluster(bar(B_PART_FULL + 2 * group + b), (used >> 1) & 1);
                     if (!ok) break;
-                    for (int m = rank * 4 + warp; m < min(left, kChunk); m += 4 * split) {
+                    for (int m = rank * 4 + w4; m < min(left, kChunk); m += 4 * split) {
                         const uint32_t row = smem_u32(stage + m * kFeat);
-                        float4 sums = make_float4(0.f, 0.f, 0.f, 0.f);
+                        float q[1][4] = {}, r[4] = {};
+                        if (a.residual) residual_of(row0 + m, r);
                         for (int p = 0; p < split; ++p) {
-                            const float4 q = staged(peer_addr(row, p), std::true_type{});
-                            sums.x += q.x; sums.y += q.y; sums.z += q.z; sums.w += q.w;
+                            float part[4];
+                            staged(peer_addr(row, p), std::true_type{}, part);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) q[0][i] += part[i];
                         }
-                        finish(c * kChunk + m, sums);
+                        finish(q);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q[0][i] += r[i];
+                        store(row0 + m, q[0]);
                     }
                     __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_EMPTY + b), lane));
+                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_EMPTY + 2 * group + b), lane));
                 }
             }
         }
         timed_out = !ok;
     }
     if (timed_out && a.status && lane == 0) atomicOr(a.status, SFB_STATUS_WAIT_TIMEOUT);
-    // ---- teardown: every warp arrives here; with a cluster no block leaves while another may still read its sums
+    // ---- teardown: every warp arrives here; in a cluster no block leaves while another may still use its shared memory
     tc_fence_before();
     __syncthreads();
-    if (split > 1) cluster_sync();
-    if (warp == 5) {
+    if (cluster > 1) cluster_sync();
+    if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * kTok);
+        tmem_dealloc<PAIR>(tmem, 2 * kTok);
     }
 }
 
@@ -609,42 +740,76 @@ bool rows_for_tma(const void* base, int64_t inner, int64_t rows, int64_t stride,
     return outer <= 1 || (outer_stride % 8 == 0 && outer_stride >= 8 && outer_stride < (1LL << 38));
 }
 
-template <int kTok, int kStages, bool BF16>
-int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int sms, cudaStream_t stream) {
-    auto kernel = linear_tcgen05_kernel<kTok, kStages, BF16>;
-    const int rc = allow_shared_memory_once(reinterpret_cast<const void*>(kernel), smem_bytes(kTok, kStages, kMaxGroups));
-    if (rc != SFB_OK) return rc;
+// How many clusters of `size` blocks of a kernel the device holds at once (0: none); asked once per kernel, device and size.
+int resident_clusters(const void* kernel, int size, int threads, int smem, int dev, int sms) {
+    struct Known { const void* kernel; int size, threads, dev, clusters; };
+    static std::mutex mu;
+    static std::vector<Known> known;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Known& k : known)
+        if (k.kernel == kernel && k.size == size && k.threads == threads && k.dev == dev) return k.clusters;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)a.split; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(units, sms / a.split) * a.split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)smem_bytes(kTok, kStages, a.groups);
+    attr.val.clusterDim.x = (unsigned)size; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(sms / size * size)); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    cudaGetLastError();  // a refusal only means "not available"
+    clusters = std::max(0, std::min(clusters, sms / size));
+    known.push_back({kernel, size, threads, dev, clusters});
+    return clusters;
+}
+
+template <typename S, bool BF16>
+int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int dev, int sms, cudaStream_t stream) {
+    auto kernel = linear_tcgen05_kernel<S, BF16>;
+    const void* k = reinterpret_cast<const void*>(kernel);
+    const int rc = allow_shared_memory_once(k, S::smem(kMaxGroups));
+    if (rc != SFB_OK) return rc;
+    const int cluster = S::kPair ? 2 : a.split, threads = kThreads + (a.row_index ? kGatherThreads : 0);
+    int resident = sms;
+    if (cluster > 1 && (resident = resident_clusters(k, cluster, threads, S::smem(kMaxGroups), dev, sms)) == 0)
+        return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(units, resident) * cluster));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)S::smem(a.groups);
     cfg.stream = stream;
-    cfg.attrs = &attr; cfg.numAttrs = a.split > 1 ? 1 : 0;
+    cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
     SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], a));
     return SFB_OK;
 }
 
 }  // namespace
 
+// Every candidate shape is priced in clocks: rounds of tiles on the busiest thread block x (its K steps x a step + a tile's
+// fixed cost).  A step takes the longer of its MMAs (2 clocks a token column) and its operands' way into shared memory, and no
+// less than the issuing thread's own chain.
 LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, int sms) {
-    LinearPlan p{};
-    // Token width: the rows of a group, twice the mean where only the mean is known, in the next power of two
-    const int64_t want = grouped ? 2 * ceil_div(rows, groups) : rows;
-    p.tokens = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
-    p.feat_tiles = ceil_div(N, (int64_t)(gated ? kFeat / 2 : kFeat));
-    const int64_t token_tiles = grouped ? std::max(std::min(groups, rows), ceil_div(rows, (int64_t)p.tokens)) : ceil_div(rows, (int64_t)p.tokens);
-    const int64_t tiles = token_tiles * p.feat_tiles, n_k = ceil_div(K, (int64_t)kStepK);
-    // Split of K: rounds of tiles x (K steps + what a tile costs besides them, in steps)
-    p.split = 1;
-    int64_t best = -1;
-    for (int s = 1; s <= kMaxSplit && s <= n_k; ++s) {
-        const int64_t cost = ceil_div(tiles, (int64_t)std::max(1, sms / s)) * (ceil_div(n_k, (int64_t)s) + (s > 1 ? 8 : 4));
-        if (best < 0 || cost < best) { best = cost; p.split = s; }
-    }
-    return p;
+    LinearPlan best{};
+    int64_t best_cost = -1;
+    const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows;
+    // only the mean of the groups is known here: a group is taken to have two standard deviations of an even draw more
+    const int64_t likely = grouped ? mean + (int64_t)(2 * std::sqrt((double)mean)) : rows;
+    auto consider = [&](int tokens, bool pair, int split) {
+        const int64_t token_tiles = (grouped ? std::min(groups, rows) : 1) * ceil_div(likely, (int64_t)tokens);
+        const int64_t feat_tiles = ceil_div(N, (int64_t)((gated ? kFeat / 2 : kFeat) * (pair ? 2 : 1)));
+        const int64_t width = std::min<int64_t>(tokens, ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16);
+        const int64_t bytes = kWBytes + width * (pair ? 64 : 128);
+        const int64_t step = std::max<int64_t>({2 * width, bytes / (pair ? 64 : 48), 400});
+        const int64_t fixed = 2500 + 20 * width + (split > 1 ? 3000 : 0);
+        const int64_t cost = ceil_div(token_tiles * feat_tiles, (int64_t)std::max(1, sms / (pair ? 2 : split))) * (ceil_div(n_k, (int64_t)split) * step + fixed);
+        if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, feat_tiles}; }
+    };
+    for (int tokens : {32, 64, 128})
+        for (int split = 1; split <= kMaxSplit && split <= n_k; ++split) consider(tokens, false, split);
+    consider(256, true, 1);
+    return best;
 }
 
 int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
@@ -663,6 +828,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     if (token_tiles * plan.feat_tiles > 0x7fffffffLL) return SFB_ERR_UNSUPPORTED;
 
     TileArgs a{};
+    a.x = in.x; a.x_stride = in.x_stride; a.K = (int)in.K;
     a.bias = in.bias; a.up_bias = in.up_bias; a.residual = in.residual; a.out = in.out;
     a.offsets = in.offsets; a.row_index = in.row_index; a.status = in.status;
     a.out_stride = in.out_stride; a.res_stride = in.res_stride; a.bias_stride = in.bias_stride; a.up_bias_stride = in.up_bias_stride;
@@ -683,24 +849,18 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
         return encode(m, base, 3, inner, outer, in.groups, row, group, 64);
     };
     const int64_t x_row = in.x_rows > 1 ? in.x_stride : ceil_div(in.K, (int64_t)8) * 8;
-    if (!encode(&maps[0], in.x, 2, in.K, in.x_rows, 1, x_row, 0, in.row_index ? 1 : a.box_rows) || !weight(&maps[1], in.w, in.w_stride)) return SFB_ERR_UNSUPPORTED;
+    if (!encode(&maps[0], in.x, 2, in.K, in.x_rows, 1, x_row, 0, a.box_rows) || !weight(&maps[1], in.w, in.w_stride)) return SFB_ERR_UNSUPPORTED;
     if (in.up) { if (!weight(&maps[2], in.up, in.up_stride)) return SFB_ERR_UNSUPPORTED; }
     else maps[2] = maps[1];
 
     const int64_t units = token_tiles * plan.feat_tiles;
     const bool bf16 = in.dtype == SFB_BF16;
-    auto go = [&](auto tok, auto stages) {
-        constexpr int kTok = decltype(tok)::value, kStages = decltype(stages)::value;
-        return bf16 ? launch_tiles<kTok, kStages, true>(maps, a, units, sms, stream) : launch_tiles<kTok, kStages, false>(maps, a, units, sms, stream);
+    auto go = [&](auto shape) {
+        using S = decltype(shape);
+        return bf16 ? launch_tiles<S, true>(maps, a, units, dev, sms, stream) : launch_tiles<S, false>(maps, a, units, dev, sms, stream);
     };
-    using std::integral_constant;
-    // about 190 KB of operands in flight whatever the width
-    switch (plan.tokens) {
-        case 32: return go(integral_constant<int, 32>{}, integral_constant<int, 9>{});
-        case 64: return go(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-        case 128: return go(integral_constant<int, 128>{}, integral_constant<int, 6>{});
-        default: return go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    }
+    if (plan.pair) return go(ShapePair{});
+    return plan.tokens == 32 ? go(Shape32{}) : plan.tokens == 64 ? go(Shape64{}) : go(Shape128{});
 }
 
 }  // namespace sfb
