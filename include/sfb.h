@@ -482,10 +482,14 @@ SFB_API int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const 
  *   row_index int32 [R] or NULL  out [R, N]
  * Rows of out outside every group are left as they were.  E <= 1024.  Offsets that leave 0 .. R are clamped, one below
  * an offset before it counts as that one, and a row index outside 0 .. X-1 reads row 0; each sets
- * SFB_STATUS_BAD_ROW_INDEX. */
+ * SFB_STATUS_BAD_ROW_INDEX.
+ * workspace (may be NULL): with a row_index and many rows a group the rows of x are first laid out in their order there,
+ * sfb_grouped_linear_workspace_bytes bytes, 16-byte aligned; without it they are gathered tile by tile, which is slower. */
+SFB_API int64_t sfb_grouped_linear_workspace_bytes(int64_t rows, int64_t K, int64_t groups, int indexed);
 SFB_API int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight,
                                const SFBTensor* up_bias, const SFBTensor* group_offsets, const SFBTensor* row_index, SFBTensor* out,
-                               int weight_layout, int dtype, int out_dtype, int activation, int32_t* status, void* stream);
+                               int weight_layout, int dtype, int out_dtype, int activation, int32_t* status, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 
 /* The top_k experts of every token and the assignments sorted by expert.
  *   logits [T, E] (F32 | BF16 | F16), E <= 1024; top_k <= min(E, 32)

@@ -196,7 +196,9 @@ def _feed_forward_protos(lib: ctypes.CDLL) -> None:
     lib.sfb_fused_linear.restype = c_int
     lib.sfb_fused_linear.argtypes = [t] * 7 + [c_int] * 4 + [c_void_p, c_void_p]
     lib.sfb_grouped_linear.restype = c_int
-    lib.sfb_grouped_linear.argtypes = [t] * 8 + [c_int] * 4 + [c_void_p, c_void_p]
+    lib.sfb_grouped_linear.argtypes = [t] * 8 + [c_int] * 4 + [c_void_p, c_void_p, c_int64, c_void_p]
+    lib.sfb_grouped_linear_workspace_bytes.restype = c_int64
+    lib.sfb_grouped_linear_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
     lib.sfb_moe_route_workspace_bytes.restype = c_int64
     lib.sfb_moe_route_workspace_bytes.argtypes = [c_int64, c_int64]
     lib.sfb_moe_route.restype = c_int

@@ -20,6 +20,8 @@ struct LinearArgs {
     int64_t rows, x_rows, K, N, groups;
     int layout, dtype, out_dtype, act;
     int* status;
+    void* workspace;  // rows * ceil(K / 8) * 16 bytes, or nullptr: room for the rows of x in the order of out
+    int64_t workspace_bytes;
 };
 int launch_linear_generic(const LinearArgs& a, cudaStream_t stream);
 // Returns SFB_ERR_UNSUPPORTED (leaving the error text alone) for types and alignments outside what TMA and the tensor cores
@@ -31,7 +33,8 @@ struct LinearPlan {
     int split;           // thread blocks that share a tile's K steps
     int64_t feat_tiles;  // tiles across the columns of out
 };
-LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, int sms);
+LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms);
+constexpr int kOrderedRows = 64;  // mean rows of a group from which a call with a row index asks for that workspace
 
 constexpr int kMaxGroups = 1024;  // groups (experts) of one call
 constexpr int kMaxTopK = 32;

@@ -103,9 +103,14 @@ int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTenso
     return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
 
+int64_t sfb_grouped_linear_workspace_bytes(int64_t rows, int64_t K, int64_t groups, int indexed) {
+    if (rows < 0 || K < 0 || groups < 1) return SFB_ERR_INVALID_ARG;
+    return indexed && rows >= kOrderedRows * groups ? rows * ceil_div(K, (int64_t)8) * 16 : 0;
+}
+
 int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight, const SFBTensor* up_bias,
                        const SFBTensor* group_offsets, const SFBTensor* row_index, SFBTensor* out, int weight_layout, int dtype, int out_dtype,
-                       int activation, int32_t* status, void* stream) {
+                       int activation, int32_t* status, void* workspace, int64_t workspace_bytes, void* stream) {
     SFB_TRACE_OP("grouped_linear", stream, "dtype %d activation %d gated %d", dtype, activation, up_weight ? 1 : 0);
     LinearArgs a{};
     if (const int rc = linear_views("grouped_linear", x, weight, bias, up_weight, up_bias, out, true, weight_layout, dtype, out_dtype, activation, &a)) return rc;
@@ -125,6 +130,8 @@ int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTen
     }
     if (a.rows == 0 || a.N == 0) return SFB_OK;
     if (a.K == 0) return fail(SFB_ERR_INVALID_ARG, "grouped_linear: K is zero");
+    a.workspace = workspace;
+    a.workspace_bytes = workspace ? workspace_bytes : 0;
     a.status = status;
     return launch_linear(a, static_cast<cudaStream_t>(stream));
 }

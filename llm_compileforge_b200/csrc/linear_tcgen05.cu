@@ -10,9 +10,8 @@
 //
 // Persistent thread blocks walk the tiles; accumulators are double-buffered in tensor memory (2 x kTok columns):
 //   warp 8      TMA producer: per 64-wide K step two boxes of 64 features, and the token rows as boxes of box_rows rows
-//   warps 10-13 with a row index, the token rows instead: 16-byte cp.async pieces, placed as the 128-byte swizzle asks.  (TMA's
-//               own row gather takes four rows an instruction and about 60 clocks for each: 4000 clocks for a K step of 256
-//               rows whose MMAs take 512.)
+//               or, with a row index, as row gathers of four rows (about 60 clocks each, whatever they bring: right for the
+//               few rows an expert has in decode; for many a pass before this kernel lays the rows out in index order)
 //   warp 9      one thread issues tcgen05.mma kind::f16 (N = tokens, K 16, four per step); the weight operand is MN-major for
 //               [K, N] storage and K-major for [N, K], straight from 128-byte-swizzled shared memory
 //   warps 0-7   epilogue, two groups of four warps that take every other 16 tokens: through a transposing buffer in shared
@@ -44,9 +43,7 @@ constexpr int kFeat = 128, kStepK = 64, kChunk = 16;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
 constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]; two for each epilogue group
-constexpr int kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 10, kGatherThreads = 128;
-constexpr int kThreads = 32 * kGatherWarp;       // without a row index
-constexpr int kGatherLag = 3;                    // K steps of gathered rows in flight behind the one being issued
+constexpr int kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;
 constexpr uint32_t kSpin = 1u << 21;
 constexpr int kMaxSplit = 8;
 
@@ -70,7 +67,7 @@ struct Shape {
     static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
     static constexpr int kStage = kWBytes + kRows * 128;
     static constexpr int smem(int groups) { return 1024 + kStages * kStage + 4 * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
-    static_assert(STAGES <= kMaxStages && STAGES > kGatherLag + 1, "pipeline depth");
+    static_assert(STAGES <= kMaxStages, "pipeline depth");
 };
 // About 160 KB of operands in flight whatever the width
 using Shape32 = Shape<32, 8, false>;
@@ -81,12 +78,12 @@ static_assert(Shape32::smem(kMaxGroups) <= 232448 && Shape64::smem(kMaxGroups) <
               ShapePair::smem(kMaxGroups) <= 232448, "shared memory of one thread block");
 
 struct TileArgs {
-    const void *x, *bias, *up_bias, *residual;
+    const void *bias, *up_bias, *residual;
     void* out;
     const int32_t *offsets, *row_index;
     int* status;
-    int64_t x_stride, out_stride, res_stride, bias_stride, up_bias_stride;
-    int rows, x_rows, N, K, n_k, groups;
+    int64_t out_stride, res_stride, bias_stride, up_bias_stride;
+    int rows, x_rows, N, n_k, groups;
     int feat_tiles;  // column tiles of out
     int box_rows;    // token rows of one TMA box
     int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair)
@@ -178,12 +175,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // bytes < 16: the rest is zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Four rows of a map whose box is one row high, side by side at dst.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int4 r) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
+                 : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
     if constexpr (PAIR) {
@@ -312,7 +309,7 @@ struct Groups {
 };
 
 template <typename S, bool BF16>
-__global__ void __launch_bounds__(kThreads + kGatherThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                       const TileArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -323,7 +320,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     const int split = PAIR ? 1 : a.split, cluster = PAIR ? 2 : split;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     const int unit = (int)blockIdx.x / cluster, n_units = (int)gridDim.x / cluster;
-    const bool gather = a.row_index != nullptr;
+    const bool gather = !PAIR && a.row_index != nullptr;  // kPair: rows of x in the order of out
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -338,8 +335,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            // the TMA producer's arrive with the bytes, and the gathering warps (of both blocks, on the leader's barrier)
-            mbar_init(bar(B_FULL + s), 1 + (gather ? kGatherThreads / 32 * (PAIR ? 2 : 1) : 0));
+            mbar_init(bar(B_FULL + s), 1);
             mbar_init(bar(B_EMPTY + s), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -402,16 +398,30 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
 
     if (warp == kTmaWarp) {
         // ============================ TMA producer ============================
-        // Lanes 0 and 1 load the weights, lane 2 + j token box j.
+        // Lanes 0 and 1 load the weights, lane 2 + j token box j; with a row index lane j the j-th four rows.
         uint32_t s = 0, ephase = 1;
         for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
             const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
             const int n0 = column0(tile) + (a.gated ? 0 : lane * 64);  // lanes 0 and 1
             const CUtensorMap* my_w = a.gated && lane == 1 ? &umap : &wmap;
-            auto boxes_of = [&](int r) { return gather ? 0 : (own_rows(tile, r) + a.box_rows - 1) / a.box_rows; };
+            auto boxes_of = [&](int r) { return gather ? (tile.rows + 3) / 4 : (own_rows(tile, r) + a.box_rows - 1) / a.box_rows; };
             const int boxes = boxes_of(rank), all = PAIR ? boxes_of(0) + boxes_of(1) : boxes;
-            const uint32_t bytes = (PAIR ? 2 : 1) * kWBytes + all * a.box_rows * 128;
+            const uint32_t bytes = (PAIR ? 2 : 1) * kWBytes + all * (gather ? 4 : a.box_rows) * 128;
             const int row0 = tile.row0 + (PAIR ? rank * half_of(tile) : 0);
+            int4 quad = make_int4(0, 0, 0, 0);
+            if (gather) {
+                int r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = 4 * lane + i;
+                    r[i] = m < tile.rows ? a.row_index[tile.row0 + m] : 0;
+                    if (r[i] < 0 || r[i] >= a.x_rows) {
+                        if (a.status) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
+                        r[i] = 0;
+                    }
+                }
+                quad = make_int4(r[0], r[1], r[2], r[3]);
+            }
             for (int k = k_first; k < k_end; ++k) {
                 if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
                 const uint32_t dst = base + s * kStage;
@@ -420,64 +430,12 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 const uint32_t full = leader_bar(B_FULL + s);
                 const int k0 = k * kStepK;
                 if (lane < 2) tma_load_3d<PAIR>(dst + lane * kHalfBytes, my_w, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
-                else if (lane - 2 < boxes) tma_load_2d<PAIR>(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, row0 + (lane - 2) * a.box_rows);
+                else if (!gather && lane - 2 < boxes) tma_load_2d<PAIR>(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, row0 + (lane - 2) * a.box_rows);
+                if (gather && lane < boxes) tma_gather4(dst + kWBytes + lane * 512, &xmap, full, k0, quad);
                 if (++s == kStages) { s = 0; ephase ^= 1; }
             }
         }
         timed_out = __any_sync(0xffffffffu, timed_out);
-    } else if (warp >= kGatherWarp) {
-        // ====================== rows of x by their index ======================
-        // Thread i copies 16-byte piece i & 7 of rows i / 8, i / 8 + 16, ...  A K step is announced kGatherLag steps after it was
-        // issued: by then its copies are usually done.  The copies are the generic proxy's and the MMA reads through the async
-        // one, so each thread fences its own before its warp arrives.
-        constexpr int kEach = S::kRows / 16;
-        const int i = threadIdx.x - kThreads, piece = i & 7;
-        uint32_t s = 0, ephase = 1, announced = 0;  // announced: stage of the next K step to announce
-        int behind = 0;                             // steps issued and not announced
-        auto announce = [&] {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_cluster(leader_bar(B_FULL + announced));
-                else mbar_arrive(bar(B_FULL + announced));
-            }
-            if (++announced == kStages) announced = 0;
-            --behind;
-        };
-        for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
-            const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
-            const int rows = own_rows(tile, rank), row0 = tile.row0 + (PAIR ? rank * half_of(tile) : 0);
-            const T* src[kEach];
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) {
-                const int m = i / 8 + 16 * j;
-                int r = m < rows ? a.row_index[row0 + m] : 0;
-                if (r < 0 || r >= a.x_rows) {
-                    if (a.status) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
-                    r = 0;
-                }
-                src[j] = static_cast<const T*>(a.x) + (int64_t)r * a.x_stride;
-            }
-            for (int k = k_first; k < k_end; ++k) {
-                if (__any_sync(0xffffffffu, !mbar_wait(bar(B_EMPTY + s), ephase))) { timed_out = true; break; }
-                const int k0 = k * kStepK + piece * 8;
-                const int bytes = max(0, min(16, (a.K - k0) * 2));
-#pragma unroll
-                for (int j = 0; j < kEach; ++j) {
-                    const int m = i / 8 + 16 * j;
-                    if (m < rows) cp_async16(base + s * kStage + kWBytes + m * 128 + ((piece ^ (m & 7)) << 4), src[j] + (bytes ? k0 : 0), bytes);
-                }
-                cp_async_commit();
-                ++behind;
-                if (behind > kGatherLag) {
-                    cp_async_wait<kGatherLag>();
-                    announce();
-                }
-                if (++s == kStages) { s = 0; ephase ^= 1; }
-            }
-        }
-        cp_async_wait<0>();
-        while (behind > 0) announce();
     } else if (warp == kMmaWarp) {
         // ============================ MMA issuer ==============================
         if (lane == 0 && (!PAIR || rank == 0)) {
@@ -704,6 +662,34 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
 }
 
+// Rows of x in the order of out: ordered[r, :] = x[row_index[r], :] for the rows that lie in a group.
+__global__ void __launch_bounds__(256) order_rows_kernel(const uint16_t* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ row_index,
+                                                         const int32_t* __restrict__ offsets, int groups, int rows, int x_rows, int K,
+                                                         uint16_t* __restrict__ ordered, int64_t ordered_stride, int* status) {
+    int first = group_offset(offsets[0], 0, rows), end = first;
+    for (int e = threadIdx.x; e < groups; e += 256) end = group_offset(offsets[e + 1], end, rows);
+    __shared__ int ends[256];
+    ends[threadIdx.x] = end;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if (threadIdx.x < o) ends[threadIdx.x] = max(ends[threadIdx.x], ends[threadIdx.x + o]);
+        __syncthreads();
+    }
+    end = ends[0];
+    for (int r = first + blockIdx.x; r < end; r += gridDim.x) {
+        int i = row_index[r];
+        if (i < 0 || i >= x_rows) {
+            if (status && threadIdx.x == 0) atomicOr(status, SFB_STATUS_BAD_ROW_INDEX);
+            i = 0;
+        }
+        const uint16_t* src = x + (int64_t)i * x_stride;
+        uint16_t* dst = ordered + (int64_t)r * ordered_stride;
+        for (int c = threadIdx.x * 8; c + 8 <= K; c += 2048) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        const int tail = K & ~7;
+        if (threadIdx.x < K - tail) dst[tail + threadIdx.x] = src[tail + threadIdx.x];
+    }
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -768,7 +754,7 @@ int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int 
     const void* k = reinterpret_cast<const void*>(kernel);
     const int rc = allow_shared_memory_once(k, S::smem(kMaxGroups));
     if (rc != SFB_OK) return rc;
-    const int cluster = S::kPair ? 2 : a.split, threads = kThreads + (a.row_index ? kGatherThreads : 0);
+    const int cluster = S::kPair ? 2 : a.split, threads = kThreads;
     int resident = sms;
     if (cluster > 1 && (resident = resident_clusters(k, cluster, threads, S::smem(kMaxGroups), dev, sms)) == 0)
         return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
@@ -790,7 +776,7 @@ int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int 
 // Every candidate shape is priced in clocks: rounds of tiles on the busiest thread block x (its K steps x a step + a tile's
 // fixed cost).  A step takes the longer of its MMAs (2 clocks a token column) and its operands' way into shared memory, and no
 // less than the issuing thread's own chain.
-LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, int sms) {
+LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
     LinearPlan best{};
     int64_t best_cost = -1;
     const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows;
@@ -801,14 +787,16 @@ LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool 
         const int64_t feat_tiles = ceil_div(N, (int64_t)((gated ? kFeat / 2 : kFeat) * (pair ? 2 : 1)));
         const int64_t width = std::min<int64_t>(tokens, ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16);
         const int64_t bytes = kWBytes + width * (pair ? 64 : 128);
-        const int64_t step = std::max<int64_t>({2 * width, bytes / (pair ? 64 : 48), 400});
+        int64_t step = std::max<int64_t>({2 * width, bytes / (pair ? 64 : 48), 400});
+        if (indexed && !pair) step = std::max(step, std::min(width, mean) / 4 * 62);
         const int64_t fixed = 2500 + 20 * width + (split > 1 ? 3000 : 0);
-        const int64_t cost = ceil_div(token_tiles * feat_tiles, (int64_t)std::max(1, sms / (pair ? 2 : split))) * (ceil_div(n_k, (int64_t)split) * step + fixed);
+        int64_t cost = ceil_div(token_tiles * feat_tiles, (int64_t)std::max(1, sms / (pair ? 2 : split))) * (ceil_div(n_k, (int64_t)split) * step + fixed);
+        if (indexed && pair) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
         if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, feat_tiles}; }
     };
     for (int tokens : {32, 64, 128})
         for (int split = 1; split <= kMaxSplit && split <= n_k; ++split) consider(tokens, false, split);
-    consider(256, true, 1);
+    if (!indexed || ordered) consider(256, true, 1);
     return best;
 }
 
@@ -823,14 +811,16 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     int dev = 0, sms = 0;
     SFB_CUDA_CHECK(cudaGetDevice(&dev));
     SFB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    const LinearPlan plan = plan_linear(in.rows, in.K, in.N, in.groups, in.offsets != nullptr, in.up != nullptr, sms);
+    // rows by their index: the pass that puts them in order needs a workspace
+    const int64_t ordered_stride = ceil_div(in.K, (int64_t)8) * 8, ordered_bytes = in.rows * ordered_stride * 2;
+    const bool can_order = in.row_index && in.workspace && in.workspace_bytes >= ordered_bytes && reinterpret_cast<uintptr_t>(in.workspace) % 16 == 0;
+    const LinearPlan plan = plan_linear(in.rows, in.K, in.N, in.groups, in.offsets != nullptr, in.up != nullptr, in.row_index != nullptr, can_order, sms);
     const int64_t token_tiles = ceil_div(in.rows, (int64_t)plan.tokens) + (in.offsets ? std::min(in.groups, in.rows) : 0);
     if (token_tiles * plan.feat_tiles > 0x7fffffffLL) return SFB_ERR_UNSUPPORTED;
 
     TileArgs a{};
-    a.x = in.x; a.x_stride = in.x_stride; a.K = (int)in.K;
     a.bias = in.bias; a.up_bias = in.up_bias; a.residual = in.residual; a.out = in.out;
-    a.offsets = in.offsets; a.row_index = in.row_index; a.status = in.status;
+    a.offsets = in.offsets; a.row_index = plan.pair ? nullptr : in.row_index; a.status = in.status;
     a.out_stride = in.out_stride; a.res_stride = in.res_stride; a.bias_stride = in.bias_stride; a.up_bias_stride = in.up_bias_stride;
     a.rows = (int)in.rows; a.x_rows = (int)in.x_rows; a.N = (int)in.N; a.n_k = (int)ceil_div(in.K, (int64_t)kStepK); a.groups = (int)in.groups;
     a.feat_tiles = (int)plan.feat_tiles; a.split = plan.split; a.act = in.act;
@@ -838,6 +828,15 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     a.block = 8;
     // one box where the rows fit one (in eights), boxes of 32 else: the last one of a group brings in at most 31 rows too many
     a.box_rows = !in.offsets && in.rows <= 32 ? (int)(ceil_div(in.rows, (int64_t)8) * 8) : 32;
+    const bool order = plan.pair && in.row_index;
+    const void* x = order ? in.workspace : in.x;
+    const int64_t x_rows = order ? in.rows : in.x_rows, x_row = order || x_rows == 1 ? ordered_stride : in.x_stride;
+    if (order) {
+        const dim3 grid((unsigned)std::min<int64_t>(in.rows, 16 * (int64_t)sms), 1);
+        order_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(in.x), in.x_stride, in.row_index, in.offsets, (int)in.groups, (int)in.rows,
+                                                    (int)in.x_rows, (int)in.K, static_cast<uint16_t*>(in.workspace), ordered_stride, in.status);
+        SFB_CUDA_CHECK(cudaGetLastError());
+    }
     // rows of out and residual in pieces of `cols` values where all of them start on one
     const int cols = a.gated ? 2 : 4, piece = cols * (a.out_f32 ? 4 : 2);
     auto pieces = [&](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % piece == 0 && stride % cols == 0; };
@@ -848,8 +847,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
         const int64_t row = outer > 1 ? stride[ri] : ceil_div(inner, (int64_t)8) * 8, group = in.groups > 1 ? stride[0] : 8;
         return encode(m, base, 3, inner, outer, in.groups, row, group, 64);
     };
-    const int64_t x_row = in.x_rows > 1 ? in.x_stride : ceil_div(in.K, (int64_t)8) * 8;
-    if (!encode(&maps[0], in.x, 2, in.K, in.x_rows, 1, x_row, 0, a.box_rows) || !weight(&maps[1], in.w, in.w_stride)) return SFB_ERR_UNSUPPORTED;
+    if (!encode(&maps[0], x, 2, in.K, x_rows, 1, x_row, 0, a.row_index ? 1 : a.box_rows) || !weight(&maps[1], in.w, in.w_stride)) return SFB_ERR_UNSUPPORTED;
     if (in.up) { if (!weight(&maps[2], in.up, in.up_stride)) return SFB_ERR_UNSUPPORTED; }
     else maps[2] = maps[1];
 

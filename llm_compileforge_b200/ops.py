@@ -553,12 +553,13 @@ def _status_ptr(status: torch.Tensor | None, device: torch.device) -> int | None
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.Tensor, bias: torch.Tensor | None = None, *,
                    activation: str = "none", up_weight: torch.Tensor | None = None, up_bias: torch.Tensor | None = None,
                    row_index: torch.Tensor | None = None, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
-                   status: torch.Tensor | None = None) -> torch.Tensor:
+                   workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`fused_linear` for rows grouped by expert: row ``r`` with ``group_offsets[e] <= r < group_offsets[e + 1]`` (int32
     ``[E + 1]``, read on the device, groups may be empty) is ``act(x[i] @ weight[e] + bias[e]) * (x[i] @ up_weight[e] + up_bias[e])``
     with ``i = row_index[r]`` (int32, one entry per row of the result) or ``i = r`` without one.  ``weight`` and ``up_weight``
     ``[E, K, N]`` with either of the last two dimensions contiguous, biases ``[E, N]``.  Rows outside every group are left as
-    they were (in a fresh result: undefined).  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
+    they were (in a fresh result: undefined).  ``workspace`` (uint8, :func:`grouped_linear_workspace_bytes`; allocated when
+    missing) holds the rows of ``x`` in the order of ``row_index`` where groups have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
     indices outside their range."""
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
@@ -577,10 +578,24 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     elif out.shape != (rows, n):
         raise ValueError(f"grouped_linear: out has shape {tuple(out.shape)}, expected {(rows, n)}")
     dev = x.device
+    if row_index is not None and x.dtype != torch.float32:
+        need = grouped_linear_workspace_bytes(rows, x.shape[1], weight.shape[0])
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace is not None and workspace.device != dev:
+        raise ValueError(f"grouped_linear: workspace on {workspace.device}, x on {dev}")
     _on(dev, _lib.load().sfb_grouped_linear, packed(x, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
         packed(up_bias, "up_bias", dev), packed(group_offsets, "group_offsets", dev), packed(row_index, "row_index", dev), packed(out, "out", dev),
-        layout, dtype_code(x.dtype), dtype_code(odt), act, _status_ptr(status, dev))
+        layout, dtype_code(x.dtype), dtype_code(odt), act, _status_ptr(status, dev), workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0)
     return out
+
+
+def grouped_linear_workspace_bytes(rows: int, k: int, groups: int, indexed: bool = True) -> int:
+    n = _lib.load().sfb_grouped_linear_workspace_bytes(int(rows), int(k), int(groups), int(bool(indexed)))
+    if n < 0:
+        raise ValueError("invalid grouped_linear workspace query")
+    return int(n)
 
 
 class MoeRouting(NamedTuple):
