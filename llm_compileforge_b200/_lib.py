@@ -242,18 +242,19 @@ def desc(t: torch.Tensor | None, what: str = "tensor"):
 _PACK = [None] + [struct.Struct("=iiii2Qq%dq" % (2 * r)).pack for r in (1, 2, 3, 4)]
 
 
-def packed(t: torch.Tensor | None, what: str, device: torch.device):
+def packed(t: torch.Tensor | None, what: str, index: int):
     """The descriptor of :func:`desc` as bytes (``None`` stays ``None``), for calls where a few microseconds of host time
-    count; the tensor must live on ``device``, a CUDA device."""
+    count; the tensor must live on CUDA device ``index``."""
     if t is None:
         return None
-    if t.device != device or not t.is_cuda:
-        raise ValueError(f"{what} must live on {device if device.type == 'cuda' else 'a CUDA device'} (libsfb has no CPU path), got {t.device}")
+    if t.get_device() != index or index < 0:  # -1: not a CUDA tensor
+        raise ValueError(f"{what} must live on {f'cuda:{index}' if index >= 0 else 'a CUDA device'} (libsfb has no CPU path), got {t.device}")
     shape = t.shape
-    if not 1 <= len(shape) <= 4:
-        raise ValueError(f"{what}: rank {len(shape)} outside 1..4")
+    rank = len(shape)
+    if not 1 <= rank <= 4:
+        raise ValueError(f"{what}: rank {rank} outside 1..4")
     p = t.data_ptr()
-    return _PACK[len(shape)](SFB_DEVICE_CUDA, len(shape), t.element_size(), 0, p, p, 0, *shape, *t.stride())
+    return _PACK[rank](SFB_DEVICE_CUDA, rank, t.element_size(), 0, p, p, 0, *shape, *t.stride())
 
 
 def check(status: int) -> None:
@@ -270,3 +271,19 @@ def check(status: int) -> None:
 
 def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# the raw handle without a Stream object around it, where this torch has that call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def call_on(index: int, fn, *args) -> None:
+    """One library call on the current stream of CUDA device ``index``, with that device current (a launch needs its
+    stream's device to be)."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)

@@ -13,7 +13,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._lib import check, current_stream, desc, dtype_code, packed
+from ._lib import call_on, check, current_stream, desc, dtype_code, packed
 
 BLOCK_SIZE = 16
 
@@ -459,27 +459,19 @@ ACTIVATIONS = {"none": _lib.SFB_ACT_NONE, "silu": _lib.SFB_ACT_SILU, "gelu": _li
                "relu": _lib.SFB_ACT_RELU}
 
 
-def _on(device: torch.device, fn, *args) -> None:
-    """One library call with ``device`` current (a launch needs its stream's device to be)."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, current_stream(device)))
-    else:
-        with torch.cuda.device(device):
-            check(fn(*args, current_stream(device)))
-
-
 def _same_type(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
     for name, t in tensors.items():
-        if t is not None and t.dtype != dtype:
+        if t is not None and t.dtype is not dtype:
             raise ValueError(f"{what}: {name} is {t.dtype}, expected {dtype}")
 
 
 def _matrix(what: str, w: torch.Tensor, like: int | None = None) -> tuple[torch.Tensor, int]:
     """A ``[.., K, N]`` weight as the library takes it: itself, or, when K is the contiguous dimension, its transpose."""
-    if w.stride(-1) == 1 and like != _lib.SFB_WEIGHT_NK:
+    stride = w.stride()
+    if stride[-1] == 1 and like != _lib.SFB_WEIGHT_NK:
         return w, _lib.SFB_WEIGHT_KN
-    if w.stride(-2) == 1 and like != _lib.SFB_WEIGHT_KN:
-        return w.transpose(-1, -2), _lib.SFB_WEIGHT_NK
+    if stride[-2] == 1 and like != _lib.SFB_WEIGHT_KN:
+        return w.mT, _lib.SFB_WEIGHT_NK
     raise ValueError(f"{what}: one of the last two dimensions of a weight must be contiguous, the same one for both weights")
 
 
@@ -511,43 +503,58 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     :data:`ACTIVATIONS`.  The result has ``x``'s type, or float32 with ``out_dtype=torch.float32``; ``out`` may be the residual
     itself.  fp32 accumulation, one rounding.  bf16 / fp16 operands whose rows are 16-byte aligned run on the tensor
     cores, all others on the CUDA cores.  ``status`` (int32, device) collects status bits."""
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
-        raise ValueError(f"fused_linear: x [..., K] and weight [K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    k, n = weight.shape
+    xs, ws, dtype = x.shape, weight.shape, x.dtype
+    if len(ws) != 2 or not xs or xs[-1] != ws[0]:
+        raise ValueError(f"fused_linear: x [..., K] and weight [K, N], got {tuple(xs)} and {tuple(ws)}")
+    k, n = ws
     act = _activation("fused_linear", activation)
-    odt = out.dtype if out is not None else out_dtype or x.dtype
-    _same_type("fused_linear", x.dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
-    _same_type("fused_linear", odt, residual=residual)
+    odt = out.dtype if out is not None else out_dtype or dtype
+    _same_type("fused_linear", dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
     if k == 0:
         raise ValueError("fused_linear: K is zero")
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    if x2.stride(-1) != 1 and k > 1:
+    flat = len(xs) == 2
+    x2 = x if flat else x.reshape(-1, k)
+    if x2.stride(1) != 1 and k > 1:
         x2 = x2.contiguous()
     w, layout = _matrix("fused_linear", weight)
     u = _matrix("fused_linear", up_weight, layout)[0] if up_weight is not None else None
-    shape = (*x.shape[:-1], n)
-    for name, t in (("out", out), ("residual", residual)):
-        if t is not None and t.shape != shape:
-            raise ValueError(f"fused_linear: {name} has shape {tuple(t.shape)}, expected {shape}")
+    shape = (*xs[:-1], n)
+    if out is not None and out.shape != shape:
+        raise ValueError(f"fused_linear: out has shape {tuple(out.shape)}, expected {shape}")
+    r2 = None
+    if residual is not None:
+        if residual.dtype is not odt or residual.shape != shape:
+            raise ValueError(f"fused_linear: residual is {residual.dtype} {tuple(residual.shape)}, expected {odt} {shape}")
+        r2 = residual if flat else residual.reshape(-1, n) if n else residual
+        if n > 1 and r2.stride(-1) != 1:
+            r2 = r2.contiguous()
     if n == 0:
-        return torch.empty(shape, dtype=odt, device=x.device) if out is None else out
-    o2 = torch.empty((x2.shape[0], n), dtype=odt, device=x.device) if out is None else _rows("fused_linear: out", out, n)
-    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, n)
-    if r2 is not None and r2.stride(-1) != 1 and n > 1:
-        r2 = r2.contiguous()
-    dev = x.device
-    _on(dev, _lib.load().sfb_fused_linear, packed(x2, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
-        packed(up_bias, "up_bias", dev), packed(r2, "residual", dev), packed(o2, "out", dev), layout, dtype_code(x.dtype), dtype_code(odt), act,
-        _status_ptr(status, dev))
-    return out if out is not None else o2.view(shape)
+        return x.new_empty(shape, dtype=odt) if out is None else out
+    o2 = x.new_empty((x2.shape[0], n), dtype=odt) if out is None else _rows("fused_linear: out", out, n)
+    dev = x.get_device()
+    call_on(dev, _lib.load().sfb_fused_linear, packed(x2, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
+            packed(up_bias, "up_bias", dev), packed(r2, "residual", dev), packed(o2, "out", dev), layout, dtype_code(dtype), dtype_code(odt), act,
+            _status_ptr(status, dev))
+    return out if out is not None else o2 if flat else o2.view(shape)
 
 
-def _status_ptr(status: torch.Tensor | None, device: torch.device) -> int | None:
+def _status_ptr(status: torch.Tensor | None, index: int) -> int | None:
     if status is None:
         return None
-    if status.dtype != torch.int32 or status.device != device or status.numel() < 1:
-        raise ValueError(f"status must be an int32 tensor on {device}")
+    if status.dtype is not torch.int32 or status.get_device() != index or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on cuda:{index}")
     return status.data_ptr()
+
+
+def _workspace(what: str, workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int | None, int]:
+    """The caller's workspace, or one of ``need`` bytes when there is none: the tensor (to keep it alive), its address and size."""
+    if workspace is None:
+        if not need:
+            return None, None, 0
+        workspace = like.new_empty(need, dtype=torch.uint8)
+    elif workspace.get_device() != like.get_device():
+        raise ValueError(f"{what}: workspace on {workspace.device}, operands on {like.device}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -561,33 +568,31 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     they were (in a fresh result: undefined).  ``workspace`` (uint8, :func:`grouped_linear_workspace_bytes`; allocated when
     missing) holds the rows of ``x`` in the order of ``row_index`` where groups have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
     indices outside their range."""
-    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[1]:
-        raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    n = weight.shape[2]
+    xs, ws, dtype = x.shape, weight.shape, x.dtype
+    if len(xs) != 2 or len(ws) != 3 or xs[1] != ws[1]:
+        raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(xs)} and {tuple(ws)}")
+    e, k, n = ws
     act = _activation("grouped_linear", activation)
-    odt = out.dtype if out is not None else out_dtype or x.dtype
-    _same_type("grouped_linear", x.dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
+    odt = out.dtype if out is not None else out_dtype or dtype
+    _same_type("grouped_linear", dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
     _same_type("grouped_linear", torch.int32, group_offsets=group_offsets, row_index=row_index)
-    if x.stride(1) != 1 and x.shape[1] > 1:
+    if x.stride(1) != 1 and k > 1:
         x = x.contiguous()
     w, layout = _matrix("grouped_linear", weight)
     u = _matrix("grouped_linear", up_weight, layout)[0] if up_weight is not None else None
-    rows = x.shape[0] if row_index is None else row_index.shape[0]
+    rows = xs[0] if row_index is None else row_index.shape[0]
     if out is None:
-        out = torch.empty((rows, n), dtype=odt, device=x.device)
+        out = x.new_empty((rows, n), dtype=odt)
     elif out.shape != (rows, n):
         raise ValueError(f"grouped_linear: out has shape {tuple(out.shape)}, expected {(rows, n)}")
-    dev = x.device
-    if row_index is not None and x.dtype != torch.float32:
-        need = grouped_linear_workspace_bytes(rows, x.shape[1], weight.shape[0])
-        if workspace is None and need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    if workspace is not None and workspace.device != dev:
-        raise ValueError(f"grouped_linear: workspace on {workspace.device}, x on {dev}")
-    _on(dev, _lib.load().sfb_grouped_linear, packed(x, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
-        packed(up_bias, "up_bias", dev), packed(group_offsets, "group_offsets", dev), packed(row_index, "row_index", dev), packed(out, "out", dev),
-        layout, dtype_code(x.dtype), dtype_code(odt), act, _status_ptr(status, dev), workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0)
+    dev = x.get_device()
+    need = 0
+    if row_index is not None and workspace is None and dtype is not torch.float32 and e:
+        need = grouped_linear_workspace_bytes(rows, k, e)
+    workspace, ws_ptr, ws_bytes = _workspace("grouped_linear", workspace, need, x)
+    call_on(dev, _lib.load().sfb_grouped_linear, packed(x, "x", dev), packed(w, "weight", dev), packed(bias, "bias", dev), packed(u, "up_weight", dev),
+            packed(up_bias, "up_bias", dev), packed(group_offsets, "group_offsets", dev), packed(row_index, "row_index", dev), packed(out, "out", dev),
+            layout, dtype_code(dtype), dtype_code(odt), act, _status_ptr(status, dev), ws_ptr, ws_bytes)
     return out
 
 
@@ -613,26 +618,22 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, wor
     over the chosen experts (``renormalize``) or over all, and the assignments sorted by expert, then token.  A logit of
     ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8,
     :func:`moe_route_workspace_bytes`) is allocated when missing."""
-    if logits.dim() != 2:
-        raise ValueError(f"moe_route: logits [T, E], got {tuple(logits.shape)}")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
+    ls = logits.shape
+    if len(ls) != 2:
+        raise ValueError(f"moe_route: logits [T, E], got {tuple(ls)}")
+    if logits.stride(1) != 1 and ls[1] > 1:
         logits = logits.contiguous()
-    (t, e), k, dev = logits.shape, int(top_k), logits.device
+    (t, e), k, dev = ls, int(top_k), logits.get_device()
     if k < 1 or k > min(e, 32):
         raise ValueError(f"moe_route: top_k {k} outside 1 .. min(experts, 32)")
-    # one allocation for the five results
-    every = torch.empty(4 * t * k + e + 1, dtype=torch.int32, device=dev)
-    ids, weights, positions, rows, offsets = every.split([t * k] * 4 + [e + 1])
-    ids, weights, positions = ids.view(t, k), weights.view(torch.float32).view(t, k), positions.view(t, k)
-    need = moe_route_workspace_bytes(t, e)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    if workspace is not None and workspace.device != dev:
-        raise ValueError(f"moe_route: workspace on {workspace.device}, logits on {dev}")
-    _on(dev, _lib.load().sfb_moe_route, packed(logits, "logits", dev), packed(ids, "expert_ids", dev), packed(weights, "weights", dev),
-        packed(offsets, "group_offsets", dev), packed(rows, "token_rows", dev), packed(positions, "positions", dev), dtype_code(logits.dtype),
-        1 if renormalize else 0, workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0)
+    ids, positions = logits.new_empty((2, t, k), dtype=torch.int32).unbind(0)
+    weights = logits.new_empty((t, k), dtype=torch.float32)
+    rows, offsets = logits.new_empty(t * k, dtype=torch.int32), logits.new_empty(e + 1, dtype=torch.int32)
+    need = moe_route_workspace_bytes(t, e) if workspace is None else 0
+    workspace, ws_ptr, ws_bytes = _workspace("moe_route", workspace, need, logits)
+    call_on(dev, _lib.load().sfb_moe_route, packed(logits, "logits", dev), packed(ids, "expert_ids", dev), packed(weights, "weights", dev),
+            packed(offsets, "group_offsets", dev), packed(rows, "token_rows", dev), packed(positions, "positions", dev), dtype_code(logits.dtype),
+            1 if renormalize else 0, ws_ptr, ws_bytes)
     return MoeRouting(ids, weights, offsets, rows, positions)
 
 
@@ -648,18 +649,19 @@ def moe_combine(y: torch.Tensor, positions: torch.Tensor, weights: torch.Tensor,
     """``out[t] = sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])``: every token's experts' rows (``y [R, H]``, the last
     :func:`grouped_linear`'s result) back to the token; ``positions`` int32 and ``weights`` float32 ``[T, top_k]`` are
     :func:`moe_route`'s.  A position of -1 adds nothing.  fp32 sums in the order of j, one rounding; ``out`` may be the residual."""
-    if y.dim() != 2 or positions.dim() != 2 or positions.shape != weights.shape:
-        raise ValueError(f"moe_combine: y [R, H], positions and weights [T, k], got {tuple(y.shape)}, {tuple(positions.shape)}, {tuple(weights.shape)}")
-    _same_type("moe_combine", torch.int32, positions=positions)
-    _same_type("moe_combine", torch.float32, weights=weights)
-    _same_type("moe_combine", y.dtype, residual=residual, out=out)
-    shape = (positions.shape[0], y.shape[1])
+    ys, ps, dtype = y.shape, positions.shape, y.dtype
+    if len(ys) != 2 or len(ps) != 2 or ps != weights.shape:
+        raise ValueError(f"moe_combine: y [R, H], positions and weights [T, k], got {tuple(ys)}, {tuple(ps)}, {tuple(weights.shape)}")
+    if positions.dtype is not torch.int32 or weights.dtype is not torch.float32:
+        raise ValueError(f"moe_combine: positions must be int32 and weights float32, got {positions.dtype} and {weights.dtype}")
+    _same_type("moe_combine", dtype, residual=residual, out=out)
+    shape = (ps[0], ys[1])
     for name, t in (("out", out), ("residual", residual)):
         if t is not None and t.shape != shape:
             raise ValueError(f"moe_combine: {name} has shape {tuple(t.shape)}, expected {shape}")
     if out is None:
-        out = torch.empty(shape, dtype=y.dtype, device=y.device)
-    dev = y.device
-    _on(dev, _lib.load().sfb_moe_combine, packed(y, "y", dev), packed(positions, "positions", dev), packed(weights, "weights", dev),
-        packed(residual, "residual", dev), packed(out, "out", dev), dtype_code(y.dtype), _status_ptr(status, dev))
+        out = y.new_empty(shape)
+    dev = y.get_device()
+    call_on(dev, _lib.load().sfb_moe_combine, packed(y, "y", dev), packed(positions, "positions", dev), packed(weights, "weights", dev),
+            packed(residual, "residual", dev), packed(out, "out", dev), dtype_code(dtype), _status_ptr(status, dev))
     return out
