@@ -4,12 +4,15 @@
 // (larger logit, lower index); their weights are exp(l - max) over the sum of the chosen ones (renormalize) or of all
 // experts.  The sort is stable (expert, then token): row of (t, e) = offsets[e] + number of tokens before t that chose e.
 //
-// One warp selects for one token: a lane holds every 32nd logit as a key whose unsigned order is the float order, and
-// top_k rounds of a warp-wide maximum take the winners.  A token chooses an expert at most once, so what a block of 128
-// tokens chose is one 128-bit mask per expert: a token's rank is a population count of the mask below it, whatever order
-// the bits were set in - the result does not depend on the order of the atomics.
-// With at most 128 tokens one launch does everything; with more, the blocks' counts go through a scan over the blocks
-// and a second launch places the rows.  Bound: launch latency for few tokens, the selection rounds for many.
+// One warp selects for one token: a lane holds every 32nd logit as a key whose unsigned order is the float order, sorted;
+// top_k rounds of a warp-wide maximum over the lanes' first keys take the winners.  16-bit logits carry their index in the
+// key's lower half (complemented: the lower index wins), so a round is one reduction; fp32 needs a second for the index.
+// A token chooses an expert at most once, so what a block of 128 tokens chose is one 128-bit mask per expert: a token's rank
+// is a population count of the mask below it, whatever order the bits were set in - the result does not depend on the order
+// of the atomics.
+// With at most 128 tokens one launch does everything; with more, a second launch adds up the blocks' counts and places the
+// rows (from 256 blocks up, where every block adding all counts would be quadratic, a scan comes in between).
+// Bound: launch latency for few tokens, the selection rounds' instructions for many.
 
 #include <algorithm>
 
@@ -18,7 +21,8 @@
 namespace sfb {
 namespace {
 
-constexpr int kRouteThreads = 512, kWarps = kRouteThreads / 32, kWords = kRouteTokens / 32;
+constexpr int kRouteThreads = 1024, kWarps = kRouteThreads / 32, kWords = kRouteTokens / 32;
+constexpr unsigned kSumBlocks = 256;  // up to here the placing blocks add the counts themselves
 
 __device__ __forceinline__ uint32_t order_key(float v) {  // 0: not a candidate
     if (!(v > -INFINITY)) return 0u;
@@ -28,12 +32,12 @@ __device__ __forceinline__ uint32_t order_key(float v) {  // 0: not a candidate
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ float exp_below(float v, float top) { return top == INFINITY ? (v == INFINITY ? 1.f : 0.f) : expf(v - top); }
 
-// Exclusive sum over s[0 .. n), n <= 2 * kRouteThreads, in place; s[n] receives the total.
+// Exclusive sum over s[0 .. n), n <= kRouteThreads, in place; s[n] receives the total.
 __device__ void block_exclusive_sum(int* s, int n) {
     __shared__ int warp_total[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int a = 2 * tid < n ? s[2 * tid] : 0, b = 2 * tid + 1 < n ? s[2 * tid + 1] : 0;
-    int sum = a + b;
+    const int own = tid < n ? s[tid] : 0;
+    int sum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -41,14 +45,12 @@ __device__ void block_exclusive_sum(int* s, int n) {
     }
     if (lane == 31) warp_total[warp] = sum;
     __syncthreads();
-    int before = sum - a - b;
-    for (int w = 0; w < warp; ++w) before += warp_total[w];
-    if (2 * tid < n) s[2 * tid] = before;
-    if (2 * tid + 1 < n) s[2 * tid + 1] = before + a;
-    if (2 * tid == n - 1) s[n] = before + a;
-    if (2 * tid + 1 == n - 1) s[n] = before + a + b;
+    const int others = __reduce_add_sync(0xffffffffu, lane < warp ? warp_total[lane] : 0);
+    if (tid < n) s[tid] = others + sum - own;
+    if (tid == n - 1) s[n] = others + sum;
     __syncthreads();
 }
+static_assert(kMaxGroups <= kRouteThreads && kWarps <= 32, "one expert a thread");
 
 __device__ __forceinline__ int mask_count(const uint32_t* m) {
     int c = 0;
@@ -75,6 +77,86 @@ __device__ void place_rows(const RouteArgs& a, const uint32_t (*mask)[kWords], c
     for (int64_t r = total + (int64_t)blockIdx.x * kRouteThreads + threadIdx.x; r < all; r += (int64_t)gridDim.x * kRouteThreads) a.token_rows[r] = -1;
 }
 
+// The dependent launch may start; what it reads it waits for.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A lane's logits lane, lane + 32, ... with their rounds of selection.
+template <typename T, int PER>
+struct Lane {
+    static constexpr bool kPacked = sizeof(T) == 2;  // key << 16 | ~index; a 16-bit float's key has 16 bits
+    uint32_t key[PER];
+    int index[kPacked ? 1 : PER];
+
+    __device__ __forceinline__ void load(const T* l, int lane, int experts) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = lane + 32 * i;
+            const float v = e < experts ? to_float(l[e]) : -INFINITY;
+            uint32_t k = order_key(v);
+            if constexpr (kPacked) {
+                if (k) k = pack(v, e);
+            } else {
+                index[i] = e;
+            }
+            key[i] = k;
+        }
+    }
+    // The 16-bit key of a 16-bit float, never 0 for a candidate (only -inf and NaNs lie below the lowest)
+    static __device__ __forceinline__ uint32_t pack(float v, int e) {
+        const T t = from_float<T>(v + 0.f);
+        uint32_t b = *reinterpret_cast<const uint16_t*>(&t);
+        b = b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
+        return b << 16 | (0xffffu - (uint32_t)e);
+    }
+    static __device__ __forceinline__ float value(uint32_t k) {
+        if constexpr (kPacked) {
+            const uint32_t b = k >> 16;
+            const uint16_t h = (uint16_t)(b & 0x8000u ? b & 0x7fffu : ~b);
+            return to_float(*reinterpret_cast<const T*>(&h));
+        } else {
+            return key_value(k);
+        }
+    }
+    // Odd-even transposition with strict comparisons: equal keys keep their order, the lower index first
+    __device__ __forceinline__ void sort() {
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+#pragma unroll
+            for (int i = r & 1; i + 1 < PER; i += 2) {
+                if constexpr (kPacked) {
+                    const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+                    key[i] = hi; key[i + 1] = lo;
+                } else {
+                    const bool swap = key[i] < key[i + 1];
+                    const uint32_t k = key[i];
+                    const int x = index[i];
+                    key[i] = swap ? key[i + 1] : k; index[i] = swap ? index[i + 1] : x;
+                    key[i + 1] = swap ? k : key[i + 1]; index[i + 1] = swap ? x : index[i + 1];
+                }
+            }
+    }
+    // The best key of the warp (0: none left) and its expert; it is taken out.
+    __device__ __forceinline__ uint32_t take(int& expert) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, key[0]);
+        bool won;
+        if constexpr (kPacked) {
+            expert = (int)(0xffffu - (m & 0xffffu));
+            won = key[0] == m;
+        } else {
+            expert = (int)__reduce_min_sync(0xffffffffu, key[0] == m ? (unsigned)index[0] : 0xffffffffu);
+            won = key[0] == m && index[0] == expert;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            key[i] = won ? (i + 1 < PER ? key[i + 1 < PER ? i + 1 : i] : 0u) : key[i];
+            if constexpr (!kPacked)
+                if (i + 1 < PER) index[i] = won ? index[i + 1 < PER ? i + 1 : i] : index[i];
+        }
+        return m;
+    }
+};
+
 template <typename T, int PER>
 __global__ void __launch_bounds__(kRouteThreads) route_select_kernel(const RouteArgs a) {
     __shared__ uint32_t mask[32 * PER][kWords];
@@ -83,41 +165,32 @@ __global__ void __launch_bounds__(kRouteThreads) route_select_kernel(const Route
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t0 = (int64_t)blockIdx.x * kRouteTokens;
     const int n_tokens = (int)min((int64_t)kRouteTokens, a.tokens - t0);
+    let_next_start();
     for (int i = threadIdx.x; i < 32 * PER * kWords; i += kRouteThreads) (&mask[0][0])[i] = 0u;
     __syncthreads();
 
     for (int t = warp; t < n_tokens; t += kWarps) {
-        const T* l = static_cast<const T*>(a.logits) + (t0 + t) * a.logits_stride;
-        uint32_t key[PER], best = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < a.experts ? order_key(to_float(l[lane + 32 * i])) : 0u;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) best = max(best, key[i]);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-        const float top_value = key_value(top);
+        Lane<T, PER> l;
+        l.load(static_cast<const T*>(a.logits) + (t0 + t) * a.logits_stride, lane, a.experts);
+        l.sort();
+        const uint32_t top = __reduce_max_sync(0xffffffffu, l.key[0]);
+        const float top_value = Lane<T, PER>::value(top);
         float sum = 0.f;
         if (!a.renormalize && top) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (key[i]) sum += exp_below(key_value(key[i]), top_value);
+                if (l.key[i]) sum += exp_below(Lane<T, PER>::value(l.key[i]), top_value);
             sum = warp_sum(sum);
         }
         int my_id = -1;
-        float my_weight = 0.f;
+        uint32_t my_key = 0;
         for (int j = 0; j < a.top_k; ++j) {
-            best = 0;
-            int at = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (key[i] > best) { best = key[i]; at = i; }  // ascending i: the lowest index of equal keys
-            const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+            int e;
+            const uint32_t m = l.take(e);
             if (!m) break;
-            const int e = (int)__reduce_min_sync(0xffffffffu, best == m ? (unsigned)(lane + 32 * at) : 0xffffffffu);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (lane + 32 * i == e) key[i] = 0u;
-            if (lane == j) { my_id = e; my_weight = exp_below(key_value(m), top_value); }
+            if (lane == j) { my_id = e; my_key = m; }
         }
+        const float my_weight = my_id >= 0 ? exp_below(Lane<T, PER>::value(my_key), top_value) : 0.f;
         if (a.renormalize) sum = warp_sum(my_weight);
         if (lane < a.top_k) {
             const int64_t o = (t0 + t) * a.top_k + lane;
@@ -162,26 +235,49 @@ __global__ void __launch_bounds__(1024) route_scan_kernel(int32_t* counts, int b
     if (p == 31) counts[(int64_t)blocks * experts + e] = before;
 }
 
-__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs a) {
+// scanned: the counts have been through route_scan_kernel; else every block adds those it needs.
+__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs a, bool scanned) {
     __shared__ uint32_t mask[kMaxGroups][kWords];
     __shared__ int16_t ids[kRouteTokens * kMaxTopK];
-    __shared__ int start[kMaxGroups + 1];
+    __shared__ int start[kMaxGroups + 1], before[kMaxGroups];
     const int64_t t0 = (int64_t)blockIdx.x * kRouteTokens;
-    const int n_tokens = (int)min((int64_t)kRouteTokens, a.tokens - t0);
+    const int n_tokens = (int)min((int64_t)kRouteTokens, a.tokens - t0), blocks = (int)gridDim.x;
     for (int i = threadIdx.x; i < a.experts * kWords; i += kRouteThreads) (&mask[0][0])[i] = 0u;
-    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] = a.counts[(int64_t)gridDim.x * a.experts + e];
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] = before[e] = 0;
     __syncthreads();
+    wait_for_previous();
     for (int i = threadIdx.x; i < n_tokens * a.top_k; i += kRouteThreads) {
         const int e = a.ids[t0 * a.top_k + i], t = i / a.top_k;
         ids[i] = (int16_t)e;
         if (e >= 0) atomicOr(&mask[e][t >> 5], 1u << (t & 31));
     }
+    if (scanned) {
+        for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+            start[e] = a.counts[(int64_t)blocks * a.experts + e];
+            before[e] = a.counts[(int64_t)blockIdx.x * a.experts + e];
+        }
+    } else {
+        // a thread adds every parts-th block's count of its expert
+        const int parts = kRouteThreads / a.experts, part = threadIdx.x / a.experts, e = threadIdx.x - part * a.experts;
+        if (part < parts) {
+            int all = 0, below = 0;
+#pragma unroll 8
+            for (int b = part; b < blocks; b += parts) {
+                const int c = a.counts[(int64_t)b * a.experts + e];
+                all += c;
+                below += b < (int)blockIdx.x ? c : 0;
+            }
+            atomicAdd(&start[e], all);
+            atomicAdd(&before[e], below);
+        }
+    }
+    __syncthreads();
     block_exclusive_sum(start, a.experts);
     const int total = start[a.experts];
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads) a.offsets[e] = start[e];
     __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] += a.counts[(int64_t)blockIdx.x * a.experts + e];
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] += before[e];
     __syncthreads();
     place_rows(a, mask, start, ids, t0, n_tokens, total);
 }
@@ -203,10 +299,20 @@ int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
     else launch_select<__half>(a, blocks, stream);
     SFB_CUDA_CHECK(cudaGetLastError());
     if (blocks == 1) return SFB_OK;
-    route_scan_kernel<<<(unsigned)ceil_div((int64_t)a.experts, (int64_t)32), 1024, 0, stream>>>(a.counts, (int)blocks, a.experts);
-    SFB_CUDA_CHECK(cudaGetLastError());
-    route_place_kernel<<<blocks, kRouteThreads, 0, stream>>>(a);
-    SFB_CUDA_CHECK(cudaGetLastError());
+    const bool scanned = blocks > kSumBlocks;
+    if (scanned) {
+        route_scan_kernel<<<(unsigned)ceil_div((int64_t)a.experts, (int64_t)32), 1024, 0, stream>>>(a.counts, (int)blocks, a.experts);
+        SFB_CUDA_CHECK(cudaGetLastError());
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its blocks start while the selecting ones end
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kRouteThreads);
+    cfg.stream = stream;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, route_place_kernel, a, scanned));
     return SFB_OK;
 }
 
