@@ -42,7 +42,7 @@ namespace {
 constexpr int kFeat = 128, kStepK = 64, kChunk = 16;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
-constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]; two for each epilogue group
+constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]
 constexpr int kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;
 constexpr uint32_t kSpin = 1u << 21;
 constexpr int kMaxSplit = 8;
@@ -58,24 +58,28 @@ enum {
     B_COUNT = B_PART_EMPTY + 4
 };
 
-// A kernel's shape: token columns of a tile, pipeline stages, whether a cluster of two shares each tile.
-template <int TOK, int STAGES, bool PAIR>
+// A kernel's shape: token columns of a tile, pipeline stages, thread blocks an SM, whether a cluster of two shares each tile.
+template <int TOK, int STAGES, int BLOCKS, bool PAIR>
 struct Shape {
-    static constexpr int kTok = TOK, kStages = STAGES;
+    static constexpr int kTok = TOK, kStages = STAGES, kBlocks = BLOCKS;
     static constexpr bool kPair = PAIR;
     static constexpr int kRows = PAIR ? TOK / 2 : TOK;  // token rows in one block's shared memory
     static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
+    static constexpr int kBuffers = TOK == 32 ? 1 : 2;  // staging buffers of an epilogue group; one where it has one chunk a tile
     static constexpr int kStage = kWBytes + kRows * 128;
-    static constexpr int smem(int groups) { return 1024 + kStages * kStage + 4 * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
-    static_assert(STAGES <= kMaxStages, "pipeline depth");
+    static constexpr int smem(int groups) { return 1024 + kStages * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
+    static_assert(STAGES <= kMaxStages, "barrier slots");
 };
-// About 160 KB of operands in flight whatever the width
-using Shape32 = Shape<32, 8, false>;
-using Shape64 = Shape<64, 7, false>;
-using Shape128 = Shape<128, 5, false>;
-using ShapePair = Shape<256, 5, true>;
-static_assert(Shape32::smem(kMaxGroups) <= 232448 && Shape64::smem(kMaxGroups) <= 232448 && Shape128::smem(kMaxGroups) <= 232448 &&
-              ShapePair::smem(kMaxGroups) <= 232448, "shared memory of one thread block");
+// Few tokens: the weights' way from HBM bounds.  Two blocks an SM share it evenly whatever the number of tiles, and one's
+// start, last tile and epilogue run beside the other's loads; 130 and 100 KB of weights on their way to an SM.
+using Shape32 = Shape<32, 4, 2, false>;
+using Shape64 = Shape<64, 3, 2, false>;
+// Many: about 160 KB of operands in flight.
+using Shape128 = Shape<128, 5, 1, false>;
+using ShapePair = Shape<256, 5, 1, true>;
+constexpr int kSmemPerBlock = 232448, kSmemPerSm = 233472;
+static_assert(Shape128::smem(kMaxGroups) <= kSmemPerBlock && ShapePair::smem(kMaxGroups) <= kSmemPerBlock &&
+              2 * (Shape32::smem(kMaxGroups) + 1024) <= kSmemPerSm && 2 * (Shape64::smem(256) + 1024) <= kSmemPerSm, "shared memory");
 
 struct TileArgs {
     const void *bias, *up_bias, *residual;
@@ -221,15 +225,17 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi,
             ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
             : "memory");
 }
+// Sixteen columns of this lane's row, waited for in the same statement: between a load and its wait nothing may touch the
+// registers, and across two statements the compiler could.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        " tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 // Shared-memory matrix descriptor words (sm_100 format): start address and leading byte offset in 16-byte units; stride byte
 // offset, version 1, 128-byte swizzle.
@@ -309,7 +315,7 @@ struct Groups {
 };
 
 template <typename S, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, S::kBlocks)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                       const TileArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -325,7 +331,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
     float* staging = reinterpret_cast<float*>(base_ptr + kStages * kStage);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + 4 * kStaging);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + 2 * S::kBuffers * kStaging);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
     int* g_off = reinterpret_cast<int*>(tmem_slot + 4);
     int* g_tiles = g_off + a.groups + 1;
@@ -333,19 +339,10 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     auto leader_bar = [&](int i) { return PAIR ? peer_addr(bar(i), 0) : bar(i); };
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(bar(B_FULL + s), 1);
-            mbar_init(bar(B_EMPTY + s), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(B_ACC_FULL + i), 1);
-            mbar_init(bar(B_ACC_EMPTY + i), kEpilogueWarps * (PAIR ? 2 : 1));
-        }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(bar(B_PART_FULL + i), 4 * split);
-            mbar_init(bar(B_PART_EMPTY + i), 4 * split);
-        }
+    if (warp == kTmaWarp) {  // one barrier a lane
+        if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &wmap : lane == 1 ? &xmap : &umap) : "memory");
+        for (int i = lane; i < B_COUNT; i += 32)
+            mbar_init(bar(i), i < B_ACC_EMPTY ? 1 : i < B_PART_FULL ? kEpilogueWarps * (PAIR ? 2 : 1) : 4 * split);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -475,179 +472,230 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         // ============================== epilogue ==============================
         const int group = warp >> 2, w4 = warp & 3;  // this group takes chunks group, group + 2, ..
         const int sync_id = 1 + group;
-        bool ok = true;
-        int it = 0, used = 0;  // chunks that this group has staged
+        float* const stage0 = staging + S::kBuffers * group * (kStaging / 4);
+        bool ok = true, gone = false;  // a warp whose wait ran out; its group then leaves together, at the next tile
+        int it = 0, used = 0;          // chunks that this group has staged
         const int cols = a.gated ? 2 : 4;  // columns of out that a lane writes for a token
         // vec: lane l holds columns cols * l ..; else l, l + 32, ..
         const int col0 = a.vec ? cols * lane : lane, col_step = a.vec ? 1 : 32;
-        for (int t = unit; t < tiles_total; t += n_units, ++it) {
-            const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
-            const int buf = it & 1, n = column0(tile) + col0;
-            float bias[4] = {}, up_bias[2] = {};
-            const T* bp = a.bias ? static_cast<const T*>(a.bias) + tile.group * a.bias_stride : nullptr;
-            const T* cp = a.up_bias ? static_cast<const T*>(a.up_bias) + tile.group * a.up_bias_stride : nullptr;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = n + i * col_step;
-                if (i < cols && c < a.N) {
-                    if (bp) bias[i] = to_float(bp[c]);
-                    if (cp && i < 2) up_bias[i] = to_float(cp[c]);
-                }
+        float bias[4] = {}, up_bias[2] = {};
+        Tile tile{};
+        int buf = 0, n = 0, chunks = 0;
+        uint32_t acc = 0;
+        // Once per tile: what does not need the accumulator, then the wait for it
+        auto release = [&] {  // the accumulator goes back: the next-but-one tile may overwrite it
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(leader_bar(B_ACC_EMPTY + buf));
+                else mbar_arrive(bar(B_ACC_EMPTY + buf));
             }
+        };
+        auto wait_accumulator = [&] {
             if (ok) ok = PAIR ? mbar_wait_cluster(bar(B_ACC_FULL + buf), (it >> 1) & 1) : mbar_wait(bar(B_ACC_FULL + buf), (it >> 1) & 1);
-            if (group_any(sync_id, !ok)) { ok = false; break; }
+            gone = group_any(sync_id, !ok);
+            if (gone) return ok = false;
             tc_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(w4 * 32) << 16) + buf * kTok;
-            const int chunks = (tile.rows + kChunk - 1) / kChunk;
-            auto release = [&] {  // the accumulator goes back: the next-but-one tile may overwrite it
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (PAIR) mbar_arrive_cluster(leader_bar(B_ACC_EMPTY + buf));
-                    else mbar_arrive(bar(B_ACC_EMPTY + buf));
-                }
-            };
             if (group >= chunks) release();
+            return true;
+        };
+        // bias, activation and gate of COUNT tokens' sums
+        auto finish = [&](auto& q, auto gated) {
+            constexpr int COUNT = sizeof(q) / sizeof(q[0]);
+            if constexpr (decltype(gated)::value) {
+                float g[2 * COUNT];
+#pragma unroll
+                for (int j = 0; j < COUNT; ++j) { g[2 * j] = q[j][0] + bias[0]; g[2 * j + 1] = q[j][1] + bias[1]; }
+                activate_all(g, a.act);
+#pragma unroll
+                for (int j = 0; j < COUNT; ++j) { q[j][0] = g[2 * j] * (q[j][2] + up_bias[0]); q[j][1] = g[2 * j + 1] * (q[j][3] + up_bias[1]); }
+            } else {
+                float h[4 * COUNT];
+#pragma unroll
+                for (int j = 0; j < 4 * COUNT; ++j) h[j] = q[j / 4][j % 4] + bias[j % 4];
+                activate_all(h, a.act);
+#pragma unroll
+                for (int j = 0; j < 4 * COUNT; ++j) q[j / 4][j % 4] = h[j];
+            }
+        };
 
-            // a token's staged sums for this lane, from the row at `addr` (of any block): its columns; with a gate those of the
-            // gate, then those of the up projection
-            auto staged = [&](uint32_t addr, auto peer, float (&q)[4]) {
-                constexpr bool P = decltype(peer)::value;
-                if (!a.vec) {
+        // A tile of 16-bit rows in whole pieces, the usual case: no branch between the loads of a chunk, and the next chunk's
+        // residual on its way while this one is worked on.  (With the choices made value by value a chunk
+        // took 1500 clocks, with a residual 5500.)
+        auto whole_pieces = [&](auto gated, auto with_residual) {
+            constexpr bool GATED = decltype(gated)::value, RES = decltype(with_residual)::value;
+            constexpr int kEach = kChunk / 4;
+            using Word = std::conditional_t<GATED, uint32_t, uint2>;
+            const bool in = n < a.N;  // N is a multiple of cols
+            const int64_t row0 = tile.row0 + group * kChunk + w4;
+            T* out = static_cast<T*>(a.out) + row0 * a.out_stride + n;
+            const T* res = RES ? static_cast<const T*>(a.residual) + row0 * a.res_stride + n : nullptr;
+            Word r[kEach];
+            auto load_residual = [&](int left) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) ld_shared<1, P>(q + i, addr + 4u * (uint32_t)(lane + 32 * i));
-                } else if (a.gated) {
-                    ld_shared<2, P>(q, addr + 8u * (uint32_t)lane);
-                    ld_shared<2, P>(q + 2, addr + 256u + 8u * (uint32_t)lane);
-                } else {
-                    ld_shared<4, P>(q, addr + 16u * (uint32_t)lane);
+                for (int i = 0; i < kEach; ++i) {
+                    r[i] = Word{};
+                    if (in && w4 + 4 * i < left) r[i] = *reinterpret_cast<const Word*>(res + 4 * i * a.res_stride);
                 }
+                res += 2 * kChunk * a.res_stride;
             };
-            // the residual of one token's columns, and their place in out
-            auto residual_of = [&](int64_t row, float (&r)[4]) {
-                if (a.out_f32) {
-                    const float* p = static_cast<const float*>(a.residual) + row * a.res_stride + n;
-                    if (!a.vec) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < cols && n + 32 * i < a.N) r[i] = p[32 * i];
-                    } else if (n < a.N) {
-                        if (a.gated) { const float2 v = *reinterpret_cast<const float2*>(p); r[0] = v.x; r[1] = v.y; }
-                        else { const float4 v = *reinterpret_cast<const float4*>(p); r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
-                    }
-                    return;
-                }
-                const T* p = static_cast<const T*>(a.residual) + row * a.res_stride + n;
-                if (!a.vec) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i < cols && n + 32 * i < a.N) r[i] = to_float(p[32 * i]);
-                } else if (n < a.N) {
-                    const uint2 u = a.gated ? make_uint2(*reinterpret_cast<const uint32_t*>(p), 0u) : *reinterpret_cast<const uint2*>(p);
-                    const float2 lo = unpack2<BF16>(u.x), hi = unpack2<BF16>(u.y);
-                    r[0] = lo.x; r[1] = lo.y; r[2] = hi.x; r[3] = hi.y;
-                }
-            };
-            auto store = [&](int64_t row, const float (&v)[4]) {
-                if (a.out_f32) {
-                    float* o = static_cast<float*>(a.out) + row * a.out_stride + n;
-                    if (!a.vec) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < cols && n + 32 * i < a.N) o[32 * i] = v[i];
-                    } else if (n < a.N) {  // N is a multiple of cols
-                        if (a.gated) *reinterpret_cast<float2*>(o) = make_float2(v[0], v[1]);
-                        else *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-                    }
-                    return;
-                }
-                T* o = static_cast<T*>(a.out) + row * a.out_stride + n;
-                if (!a.vec) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i < cols && n + 32 * i < a.N) o[32 * i] = from_float<T>(v[i]);
-                } else if (n < a.N) {
-                    if (a.gated) *reinterpret_cast<uint32_t*>(o) = pack2<BF16>(v[0], v[1]);
-                    else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
-                }
-            };
-            // COUNT tokens' sums -> bias, activation, gate
-            auto finish = [&](auto& q) {
-                constexpr int COUNT = sizeof(q) / sizeof(q[0]);
-                if (a.gated) {
-                    float g[2 * COUNT];
-#pragma unroll
-                    for (int j = 0; j < COUNT; ++j) { g[2 * j] = q[j][0] + bias[0]; g[2 * j + 1] = q[j][1] + bias[1]; }
-                    activate_all(g, a.act);
-#pragma unroll
-                    for (int j = 0; j < COUNT; ++j) { q[j][0] = g[2 * j] * (q[j][2] + up_bias[0]); q[j][1] = g[2 * j + 1] * (q[j][3] + up_bias[1]); }
-                } else {
-                    float h[4 * COUNT];
-#pragma unroll
-                    for (int j = 0; j < 4 * COUNT; ++j) h[j] = q[j / 4][j % 4] + bias[j % 4];
-                    activate_all(h, a.act);
-#pragma unroll
-                    for (int j = 0; j < 4 * COUNT; ++j) q[j / 4][j % 4] = h[j];
-                }
-            };
-
+            if constexpr (RES) load_residual(tile.rows - group * kChunk);
+            if (!wait_accumulator()) return;
             for (int c = group; c < chunks; c += 2, ++used) {
+                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * (kStaging / 4) : 0);
                 float v[kChunk];
                 tmem_ld16(acc + c * kChunk, v);
                 if (c + 2 >= chunks) release();
-                const int b = used & 1, left = tile.rows - c * kChunk;
-                const int64_t row0 = tile.row0 + c * kChunk;
-                float* stage = staging + (2 * group + b) * (kStaging / 4);
-                if (split == 1) {
-                    constexpr int kEach = kChunk / 4;
-                    float q[kEach][4], r[kEach][4];
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
-                    if (a.residual) {
+                for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                // one barrier a chunk: a buffer is written again two chunks on, after the next chunk's barrier (with one chunk a
+                // tile: after the next tile's)
+                group_sync(sync_id);
+                float q[kEach][4];
 #pragma unroll
-                        for (int i = 0; i < kEach; ++i)
-                            if (w4 + 4 * i < left) residual_of(row0 + w4 + 4 * i, r[i]);
+                for (int i = 0; i < kEach; ++i) {
+                    const uint32_t row = smem_u32(stage + (w4 + 4 * i) * kFeat);
+                    if constexpr (GATED) {
+                        ld_shared<2, false>(q[i], row + 8u * (uint32_t)lane);
+                        ld_shared<2, false>(q[i] + 2, row + 256u + 8u * (uint32_t)lane);
+                    } else {
+                        ld_shared<4, false>(q[i], row + 16u * (uint32_t)lane);
                     }
-                    group_sync(sync_id);  // one barrier a chunk: a buffer is written again two chunks on, after the next chunk's barrier
+                }
+                finish(q, gated);
+                if constexpr (RES) {
 #pragma unroll
-                    for (int i = 0; i < kEach; ++i) staged(smem_u32(stage + (w4 + 4 * i) * kFeat), std::false_type{}, q[i]);
-                    finish(q);
-                    if (a.residual) {
-#pragma unroll
-                        for (int i = 0; i < 4 * kEach; ++i) q[i / 4][i % 4] += r[i / 4][i % 4];
+                    for (int i = 0; i < kEach; ++i) {
+                        if constexpr (GATED) {
+                            const float2 f = unpack2<BF16>(r[i]);
+                            q[i][0] += f.x; q[i][1] += f.y;
+                        } else {
+                            const float2 f = unpack2<BF16>(r[i].x), g = unpack2<BF16>(r[i].y);
+                            q[i][0] += f.x; q[i][1] += f.y; q[i][2] += g.x; q[i][3] += g.y;
+                        }
                     }
+                    load_residual(tile.rows - (c + 2) * kChunk);
+                }
+                const int left = tile.rows - c * kChunk;
 #pragma unroll
-                    for (int i = 0; i < kEach; ++i)
-                        if (w4 + 4 * i < left) store(row0 + w4 + 4 * i, q[i]);
-                } else {
-                    ok = ok && mbar_wait_cluster(bar(B_PART_EMPTY + 2 * group + b), ((used >> 1) & 1) ^ 1);
+                for (int i = 0; i < kEach; ++i)
+                    if (in && w4 + 4 * i < left) {
+                        if constexpr (GATED) *reinterpret_cast<uint32_t*>(out + 4 * i * a.out_stride) = pack2<BF16>(q[i][0], q[i][1]);
+                        else *reinterpret_cast<uint2*>(out + 4 * i * a.out_stride) = make_uint2(pack2<BF16>(q[i][0], q[i][1]), pack2<BF16>(q[i][2], q[i][3]));
+                    }
+                out += 2 * kChunk * a.out_stride;
+            }
+        };
+
+        // Every other form (fp32 out, rows that do not divide into pieces, K split over a cluster), one token at a time
+        auto residual_of = [&](int64_t row, float (&r)[4]) {
+            auto each = [&](auto* p) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < cols && n + i * col_step < a.N) r[i] = to_float(p[row * a.res_stride + n + i * col_step]);
+            };
+            if (!a.residual) return;
+            if (a.out_f32) each(static_cast<const float*>(a.residual));
+            else each(static_cast<const T*>(a.residual));
+        };
+        auto one_token = [&](float (&q)[1][4], const float (&r)[4], int64_t row) {
+            if (a.gated) finish(q, std::true_type{});
+            else finish(q, std::false_type{});
+            auto each = [&](auto* p) {
+                using O = std::remove_pointer_t<decltype(p)>;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < cols && n + i * col_step < a.N) p[row * a.out_stride + n + i * col_step] = from_float<O>(a.residual ? q[0][i] + r[i] : q[0][i]);
+            };
+            if (a.out_f32) each(static_cast<float*>(a.out));
+            else each(static_cast<T*>(a.out));
+        };
+        // a token's staged sums for this lane, from the row at `addr` (of any block): its columns; with a gate those of the gate,
+        // then those of the up projection
+        auto staged = [&](uint32_t addr, auto peer, float (&q)[4]) {
+            constexpr bool P = decltype(peer)::value;
+            if (!a.vec) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ld_shared<1, P>(q + i, addr + 4u * (uint32_t)(lane + 32 * i));
+            } else if (a.gated) {
+                ld_shared<2, P>(q, addr + 8u * (uint32_t)lane);
+                ld_shared<2, P>(q + 2, addr + 256u + 8u * (uint32_t)lane);
+            } else {
+                ld_shared<4, P>(q, addr + 16u * (uint32_t)lane);
+            }
+        };
+        auto any_form = [&] {
+            float r[4] = {};
+            const int first = (split > 1 ? rank * 4 : 0) + w4;  // this warp's first token of a chunk
+            if (group * kChunk + first < tile.rows) residual_of(tile.row0 + group * kChunk + first, r);
+            if (!wait_accumulator()) return;
+            for (int c = group; c < chunks; c += 2, ++used) {
+                const int b = S::kBuffers == 2 ? used & 1 : 0, turn = S::kBuffers == 2 ? used >> 1 : used, left = tile.rows - c * kChunk;
+                const uint32_t part_full = bar(B_PART_FULL + 2 * group + b), part_empty = bar(B_PART_EMPTY + 2 * group + b);
+                float* stage = stage0 + b * (kStaging / 4);
+                float v[kChunk];
+                tmem_ld16(acc + c * kChunk, v);
+                if (c + 2 >= chunks) release();
+                if (split > 1) {
+                    ok = ok && mbar_wait_cluster(part_empty, (turn & 1) ^ 1);
                     if (!ok) break;
+                }
 #pragma unroll
-                    for (int i = 0; i < kChunk; ++i)
-                        if (i < left) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                for (int i = 0; i < kChunk; ++i)
+                    if (i < left) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                if (split > 1) {
                     __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_FULL + 2 * group + b), lane));
-                    ok = mbar_wait_cluster(bar(B_PART_FULL + 2 * group + b), (used >> 1) & 1);
+                    if (lane < split) mbar_arrive_cluster(peer_addr(part_full, lane));
+                    ok = mbar_wait_cluster(part_full, turn & 1);
                     if (!ok) break;
-                    for (int m = rank * 4 + w4; m < min(left, kChunk); m += 4 * split) {
-                        const uint32_t row = smem_u32(stage + m * kFeat);
-                        float q[1][4] = {}, r[4] = {};
-                        if (a.residual) residual_of(row0 + m, r);
+                } else {
+                    group_sync(sync_id);
+                }
+                for (int m = first; m < min(left, kChunk); m += 4 * split) {
+                    const uint32_t row = smem_u32(stage + m * kFeat);
+                    float q[1][4] = {};
+                    if (m != first) residual_of(tile.row0 + c * kChunk + m, r);
+                    if (split == 1) {
+                        staged(row, std::false_type{}, q[0]);
+                    } else {
                         for (int p = 0; p < split; ++p) {
                             float part[4];
                             staged(peer_addr(row, p), std::true_type{}, part);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) q[0][i] += part[i];
                         }
-                        finish(q);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q[0][i] += r[i];
-                        store(row0 + m, q[0]);
                     }
+                    one_token(q, r, tile.row0 + c * kChunk + m);
+                }
+                if (c + 2 < chunks && (c + 2) * kChunk + first < tile.rows) residual_of(tile.row0 + (c + 2) * kChunk + first, r);
+                if (split > 1) {
                     __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(bar(B_PART_EMPTY + 2 * group + b), lane));
+                    if (lane < split) mbar_arrive_cluster(peer_addr(part_empty, lane));
                 }
             }
+        };
+
+        const bool whole = a.vec && !a.out_f32 && split == 1;
+        for (int t = unit; t < tiles_total && !gone; t += n_units, ++it) {
+            tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+            buf = it & 1;
+            n = column0(tile) + col0;
+            chunks = (tile.rows + kChunk - 1) / kChunk;
+            acc = tmem + ((uint32_t)(w4 * 32) << 16) + buf * kTok;
+            const T* bp = a.bias ? static_cast<const T*>(a.bias) + tile.group * a.bias_stride : nullptr;
+            const T* cp = a.up_bias ? static_cast<const T*>(a.up_bias) + tile.group * a.up_bias_stride : nullptr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = n + i * col_step;
+                const bool in = i < cols && c < a.N;
+                bias[i] = bp && in ? to_float(bp[c]) : 0.f;
+                if (i < 2) up_bias[i] = cp && in ? to_float(cp[c]) : 0.f;
+            }
+            if (!whole) any_form();
+            else if (a.gated && a.residual) whole_pieces(std::true_type{}, std::true_type{});
+            else if (a.gated) whole_pieces(std::true_type{}, std::false_type{});
+            else if (a.residual) whole_pieces(std::false_type{}, std::true_type{});
+            else whole_pieces(std::false_type{}, std::false_type{});
         }
         timed_out = !ok;
     }
