@@ -31,10 +31,11 @@ struct LinearPlan {
     int tokens;          // rows of out in a tile, at most
     int pair;            // 1: a cluster of two thread blocks on each tile (256 features)
     int split;           // thread blocks that share a tile's K steps
+    int order;           // 1: rows of x are put in the order of out first
     int64_t feat_tiles;  // tiles across the columns of out
 };
 LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms);
-constexpr int kOrderedRows = 64;  // mean rows of a group from which a call with a row index asks for that workspace
+constexpr int kOrderedRows = 16;  // mean rows of a group from which a call with a row index asks for that workspace
 
 constexpr int kMaxGroups = 1024;  // groups (experts) of one call
 constexpr int kMaxTopK = 32;

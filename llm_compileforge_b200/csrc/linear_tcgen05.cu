@@ -786,12 +786,11 @@ int resident_clusters(const void* kernel, int size, int threads, int smem, int d
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)size; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(sms / size * size)); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.gridDim = dim3((unsigned)(2 * sms / size * size)); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)smem;
     cfg.attrs = &attr; cfg.numAttrs = 1;
     int clusters = 0;
     if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
     cudaGetLastError();  // a refusal only means "not available"
-    clusters = std::max(0, std::min(clusters, sms / size));
     known.push_back({kernel, size, threads, dev, clusters});
     return clusters;
 }
@@ -803,7 +802,7 @@ int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int 
     const int rc = allow_shared_memory_once(k, S::smem(kMaxGroups));
     if (rc != SFB_OK) return rc;
     const int cluster = S::kPair ? 2 : a.split, threads = kThreads;
-    int resident = sms;
+    int resident = sms * S::kBlocks;
     if (cluster > 1 && (resident = resident_clusters(k, cluster, threads, S::smem(kMaxGroups), dev, sms)) == 0)
         return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
     cudaLaunchConfig_t cfg{};
@@ -830,21 +829,24 @@ LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool 
     const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows;
     // only the mean of the groups is known here: a group is taken to have two standard deviations of an even draw more
     const int64_t likely = grouped ? mean + (int64_t)(2 * std::sqrt((double)mean)) : rows;
-    auto consider = [&](int tokens, bool pair, int split) {
+    auto consider = [&](int tokens, bool pair, int split, bool order) {
         const int64_t token_tiles = (grouped ? std::min(groups, rows) : 1) * ceil_div(likely, (int64_t)tokens);
         const int64_t feat_tiles = ceil_div(N, (int64_t)((gated ? kFeat / 2 : kFeat) * (pair ? 2 : 1)));
         const int64_t width = std::min<int64_t>(tokens, ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16);
         const int64_t bytes = kWBytes + width * (pair ? 64 : 128);
         int64_t step = std::max<int64_t>({2 * width, bytes / (pair ? 64 : 48), 400});
-        if (indexed && !pair) step = std::max(step, std::min(width, mean) / 4 * 62);
+        if (indexed && !order) step = std::max(step, std::min(width, mean) / 4 * 62);
         const int64_t fixed = 2500 + 20 * width + (split > 1 ? 3000 : 0);
-        int64_t cost = ceil_div(token_tiles * feat_tiles, (int64_t)std::max(1, sms / (pair ? 2 : split))) * (ceil_div(n_k, (int64_t)split) * step + fixed);
-        if (indexed && pair) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
-        if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, feat_tiles}; }
+        const int64_t slots = std::max(1, sms * (tokens <= 64 ? 2 : 1) / (pair ? 2 : split));
+        int64_t cost = ceil_div(token_tiles * feat_tiles, slots) * (ceil_div(n_k, (int64_t)split) * step + fixed);
+        if (order) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
+        if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, feat_tiles}; }
     };
-    for (int tokens : {32, 64, 128})
-        for (int split = 1; split <= kMaxSplit && split <= n_k; ++split) consider(tokens, false, split);
-    if (!indexed || ordered) consider(256, true, 1);
+    for (int order = 0; order <= (indexed && ordered ? 1 : 0); ++order) {
+        for (int tokens : {32, 64, 128})
+            for (int split = 1; split <= kMaxSplit && split <= n_k; ++split) consider(tokens, false, split, order);
+        if (!indexed || order) consider(256, true, 1, order);
+    }
     return best;
 }
 
@@ -868,7 +870,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
 
     TileArgs a{};
     a.bias = in.bias; a.up_bias = in.up_bias; a.residual = in.residual; a.out = in.out;
-    a.offsets = in.offsets; a.row_index = plan.pair ? nullptr : in.row_index; a.status = in.status;
+    a.offsets = in.offsets; a.row_index = plan.order ? nullptr : in.row_index; a.status = in.status;
     a.out_stride = in.out_stride; a.res_stride = in.res_stride; a.bias_stride = in.bias_stride; a.up_bias_stride = in.up_bias_stride;
     a.rows = (int)in.rows; a.x_rows = (int)in.x_rows; a.N = (int)in.N; a.n_k = (int)ceil_div(in.K, (int64_t)kStepK); a.groups = (int)in.groups;
     a.feat_tiles = (int)plan.feat_tiles; a.split = plan.split; a.act = in.act;
@@ -876,7 +878,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     a.block = 8;
     // one box where the rows fit one (in eights), boxes of 32 else: the last one of a group brings in at most 31 rows too many
     a.box_rows = !in.offsets && in.rows <= 32 ? (int)(ceil_div(in.rows, (int64_t)8) * 8) : 32;
-    const bool order = plan.pair && in.row_index;
+    const bool order = plan.order;
     const void* x = order ? in.workspace : in.x;
     const int64_t x_rows = order ? in.rows : in.x_rows, x_row = order || x_rows == 1 ? ordered_stride : in.x_stride;
     if (order) {
