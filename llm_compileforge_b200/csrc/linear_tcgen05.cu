@@ -20,9 +20,9 @@
 // Many rows a group (kPair): a cluster of two thread blocks owns 256 features x 256 tokens with cta_group::2 MMAs (M 256): each
 // block loads its 128 features and half of the tokens, the leader's MMAs read both, each block's tensor memory receives its
 // own features.
-// Few tiles (decode): a cluster of up to eight thread blocks shares a tile, each taking a part of K; the parts meet in the
-// epilogue through distributed shared memory, summed in the order of the ranks - no workspace, no atomics, the same bits
-// every time.
+// Few tiles (decode): a cluster of up to eight thread blocks owns one tile, each taking a part of K; every block lays its sums
+// into its own operand buffers, by then free, and after a cluster barrier adds its share of the tokens over all blocks' shared
+// memory in the order of the ranks - no workspace, no atomics, the same bits every time.
 // Group offsets are read on the device; each thread block lays the groups' tiles out in shared memory before it starts.
 // Every wait is bounded; one that runs out sets SFB_STATUS_WAIT_TIMEOUT and the block leaves through the common teardown.
 
@@ -53,9 +53,7 @@ enum {
     B_EMPTY = kMaxStages,
     B_ACC_FULL = 2 * kMaxStages,
     B_ACC_EMPTY = B_ACC_FULL + 2,
-    B_PART_FULL = B_ACC_EMPTY + 2,   // per epilogue group and buffer: a chunk's partial sums lie in every block's buffer
-    B_PART_EMPTY = B_PART_FULL + 4,  // every block has read the chunk
-    B_COUNT = B_PART_EMPTY + 4
+    B_COUNT = B_ACC_EMPTY + 2
 };
 
 // A kernel's shape: token columns of a tile, pipeline stages, thread blocks an SM, whether a cluster of two shares each tile.
@@ -68,7 +66,7 @@ struct Shape {
     static constexpr int kBuffers = TOK == 32 ? 1 : 2;  // staging buffers of an epilogue group; one where it has one chunk a tile
     static constexpr int kStage = kWBytes + kRows * 128;
     static constexpr int smem(int groups) { return 1024 + kStages * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
-    static_assert(STAGES <= kMaxStages, "barrier slots");
+    static_assert(STAGES <= kMaxStages && TOK * kFeat * 4 <= STAGES * kStage + 2 * kBuffers * kStaging, "barrier slots; room for a tile's sums");
 };
 // Few tokens: the weights' way from HBM bounds.  Two blocks an SM share it evenly whatever the number of tiles, and one's
 // start, last tile and epilogue run beside the other's loads; 130 and 100 KB of weights on their way to an SM.
@@ -90,7 +88,7 @@ struct TileArgs {
     int rows, x_rows, N, n_k, groups;
     int feat_tiles;  // column tiles of out
     int box_rows;    // token rows of one TMA box
-    int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair)
+    int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair); above 1 one tile a cluster
     int block;       // token tiles that run together through the feature tiles (L2 reuse of x and W)
     int act;
     bool gated, nk, out_f32, vec;
@@ -342,7 +340,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     if (warp == kTmaWarp) {  // one barrier a lane
         if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &wmap : lane == 1 ? &xmap : &umap) : "memory");
         for (int i = lane; i < B_COUNT; i += 32)
-            mbar_init(bar(i), i < B_ACC_EMPTY ? 1 : i < B_PART_FULL ? kEpilogueWarps * (PAIR ? 2 : 1) : 4 * split);
+            mbar_init(bar(i), i < B_ACC_EMPTY ? 1 : kEpilogueWarps * (PAIR ? 2 : 1));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -379,7 +377,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (cluster > 1) cluster_sync();  // the other blocks' barriers exist before anything is sent to them
+    if constexpr (PAIR) cluster_sync();  // the other block's barriers exist before anything is sent to them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const Groups groups{g_off, g_tiles, a.groups};
@@ -625,58 +623,56 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
         };
         auto any_form = [&] {
-            float r[4] = {};
-            const int first = (split > 1 ? rank * 4 : 0) + w4;  // this warp's first token of a chunk
-            if (group * kChunk + first < tile.rows) residual_of(tile.row0 + group * kChunk + first, r);
             if (!wait_accumulator()) return;
             for (int c = group; c < chunks; c += 2, ++used) {
-                const int b = S::kBuffers == 2 ? used & 1 : 0, turn = S::kBuffers == 2 ? used >> 1 : used, left = tile.rows - c * kChunk;
-                const uint32_t part_full = bar(B_PART_FULL + 2 * group + b), part_empty = bar(B_PART_EMPTY + 2 * group + b);
-                float* stage = stage0 + b * (kStaging / 4);
+                const int left = tile.rows - c * kChunk;
+                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * (kStaging / 4) : 0);
                 float v[kChunk];
                 tmem_ld16(acc + c * kChunk, v);
                 if (c + 2 >= chunks) release();
-                if (split > 1) {
-                    ok = ok && mbar_wait_cluster(part_empty, (turn & 1) ^ 1);
-                    if (!ok) break;
-                }
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i)
-                    if (i < left) stage[i * kFeat + w4 * 32 + lane] = v[i];
-                if (split > 1) {
-                    __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(part_full, lane));
-                    ok = mbar_wait_cluster(part_full, turn & 1);
-                    if (!ok) break;
-                } else {
-                    group_sync(sync_id);
-                }
-                for (int m = first; m < min(left, kChunk); m += 4 * split) {
-                    const uint32_t row = smem_u32(stage + m * kFeat);
-                    float q[1][4] = {};
-                    if (m != first) residual_of(tile.row0 + c * kChunk + m, r);
-                    if (split == 1) {
-                        staged(row, std::false_type{}, q[0]);
-                    } else {
-                        for (int p = 0; p < split; ++p) {
-                            float part[4];
-                            staged(peer_addr(row, p), std::true_type{}, part);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) q[0][i] += part[i];
-                        }
-                    }
+                for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                group_sync(sync_id);
+                for (int m = w4; m < min(left, kChunk); m += 4) {
+                    float q[1][4], r[4] = {};
+                    residual_of(tile.row0 + c * kChunk + m, r);
+                    staged(smem_u32(stage + m * kFeat), std::false_type{}, q[0]);
                     one_token(q, r, tile.row0 + c * kChunk + m);
-                }
-                if (c + 2 < chunks && (c + 2) * kChunk + first < tile.rows) residual_of(tile.row0 + (c + 2) * kChunk + first, r);
-                if (split > 1) {
-                    __syncwarp();
-                    if (lane < split) mbar_arrive_cluster(peer_addr(part_empty, lane));
                 }
             }
         };
+        // K split: this block's sums into its own shared memory, then its share of the tokens over everyone's
+        auto split_form = [&] {
+            const bool there = wait_accumulator();
+            float* sums = reinterpret_cast<float*>(base_ptr);  // all MMAs are done: the operands' room is free
+            for (int c = group; there && c < chunks; c += 2) {
+                float v[kChunk];
+                tmem_ld16(acc + c * kChunk, v);
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                    if (c * kChunk + i < tile.rows) sums[(c * kChunk + i) * kFeat + w4 * 32 + lane] = v[i];
+            }
+            int m = rank * kEpilogueWarps + warp;
+            float r[4] = {};
+            if (m < tile.rows) residual_of(tile.row0 + m, r);
+            cluster_sync();  // (1)
+            for (; there && m < tile.rows; m += split * kEpilogueWarps) {
+                float q[1][4] = {}, part[kMaxSplit][4];
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p)
+                    if (p < split) staged(peer_addr(smem_u32(sums + m * kFeat), p), std::true_type{}, part[p]);
+#pragma unroll
+                for (int p = 0; p < kMaxSplit; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (p < split) q[0][i] += part[p][i];
+                if (m >= split * kEpilogueWarps) residual_of(tile.row0 + m, r);
+                one_token(q, r, tile.row0 + m);
+            }
+        };
 
-        const bool whole = a.vec && !a.out_f32 && split == 1;
-        for (int t = unit; t < tiles_total && !gone; t += n_units, ++it) {
+        const bool whole = a.vec && !a.out_f32;
+        for (int t = unit; t < tiles_total && !gone; t += n_units, ++it) {  // (split: at most once)
             tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
             buf = it & 1;
             n = column0(tile) + col0;
@@ -691,7 +687,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 bias[i] = bp && in ? to_float(bp[c]) : 0.f;
                 if (i < 2) up_bias[i] = cp && in ? to_float(cp[c]) : 0.f;
             }
-            if (!whole) any_form();
+            if (split > 1) split_form();
+            else if (!whole) any_form();
             else if (a.gated && a.residual) whole_pieces(std::true_type{}, std::true_type{});
             else if (a.gated) whole_pieces(std::true_type{}, std::false_type{});
             else if (a.residual) whole_pieces(std::false_type{}, std::true_type{});
@@ -701,6 +698,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
     if (timed_out && a.status && lane == 0) atomicOr(a.status, SFB_STATUS_WAIT_TIMEOUT);
     // ---- teardown: every warp arrives here; in a cluster no block leaves while another may still use its shared memory
+    __syncwarp();
+    if (split > 1 && (warp >= kEpilogueWarps || unit >= tiles_total)) cluster_sync();  // (1), where not passed above
     tc_fence_before();
     __syncthreads();
     if (cluster > 1) cluster_sync();
@@ -809,7 +808,7 @@ int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int 
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)cluster; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(units, resident) * cluster));
+    cfg.gridDim = dim3((unsigned)((a.split > 1 ? units : std::min<int64_t>(units, resident)) * cluster));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)S::smem(a.groups);
     cfg.stream = stream;
