@@ -32,6 +32,7 @@ struct LinearPlan {
     int pair;            // 1: a cluster of two thread blocks on each tile (256 features)
     int split;           // thread blocks that share a tile's K steps
     int order;           // 1: rows of x are put in the order of out first
+    int blocks_an_sm;    // 1 or 2 resident thread blocks
     int64_t feat_tiles;  // tiles across the columns of out
 };
 LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms);

@@ -56,28 +56,35 @@ enum {
     B_COUNT = B_ACC_EMPTY + 2
 };
 
-// A kernel's shape: token columns of a tile, pipeline stages, thread blocks an SM, whether a cluster of two shares each tile.
-template <int TOK, int STAGES, int BLOCKS, bool PAIR>
+// A kernel's shape: token columns of a tile, thread blocks an SM, whether a cluster of two shares each tile.  The number of
+// pipeline stages follows from the shared memory that a launch gives a block.
+template <int TOK, int BLOCKS, bool PAIR>
 struct Shape {
-    static constexpr int kTok = TOK, kStages = STAGES, kBlocks = BLOCKS;
+    static constexpr int kTok = TOK, kBlocks = BLOCKS;
     static constexpr bool kPair = PAIR;
     static constexpr int kRows = PAIR ? TOK / 2 : TOK;  // token rows in one block's shared memory
     static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
     static constexpr int kBuffers = TOK == 32 ? 1 : 2;  // staging buffers of an epilogue group; one where it has one chunk a tile
     static constexpr int kStage = kWBytes + kRows * 128;
-    static constexpr int smem(int groups) { return 1024 + kStages * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
-    static_assert(STAGES <= kMaxStages && TOK * kFeat * 4 <= STAGES * kStage + 2 * kBuffers * kStaging, "barrier slots; room for a tile's sums");
+    static constexpr int smem(int stages, int groups) { return 1024 + stages * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
+    static constexpr int stages(int budget, int groups) {
+        const int n = (budget - smem(0, groups)) / kStage;
+        return n < kMaxStages ? n : kMaxStages;
+    }
 };
-// Few tokens: the weights' way from HBM bounds.  Two blocks an SM share it evenly whatever the number of tiles, and one's
-// start, last tile and epilogue run beside the other's loads; 130 and 100 KB of weights on their way to an SM.
-using Shape32 = Shape<32, 4, 2, false>;
-using Shape64 = Shape<64, 3, 2, false>;
-// Many: about 160 KB of operands in flight.
-using Shape128 = Shape<128, 5, 1, false>;
-using ShapePair = Shape<256, 5, 1, true>;
-constexpr int kSmemPerBlock = 232448, kSmemPerSm = 233472;
-static_assert(Shape128::smem(kMaxGroups) <= kSmemPerBlock && ShapePair::smem(kMaxGroups) <= kSmemPerBlock &&
-              2 * (Shape32::smem(kMaxGroups) + 1024) <= kSmemPerSm && 2 * (Shape64::smem(256) + 1024) <= kSmemPerSm, "shared memory");
+// Few tokens: the weights' way from HBM bounds.  With more tiles than SMs two blocks an SM share it evenly whatever the number
+// of tiles, and one's start, last tile and epilogue run beside the other's loads.
+using Shape32 = Shape<32, 2, false>;
+using Shape64 = Shape<64, 2, false>;
+using Shape128 = Shape<128, 1, false>;
+using ShapePair = Shape<256, 1, true>;
+constexpr int kSmemPerBlock = 232448, kSmemPerHalf = 233472 / 2 - 1024;  // of one block an SM, of each of two
+template <typename S>
+constexpr bool fits() {  // a pipeline at all, and room for a tile's sums in it
+    const int n = S::stages(S::kBlocks == 2 ? kSmemPerHalf : kSmemPerBlock, kMaxGroups);
+    return n >= 2 && S::kTok * kFeat * 4 <= n * S::kStage * (S::kPair ? 2 : 1);
+}
+static_assert(fits<Shape32>() && fits<Shape64>() && fits<Shape128>() && fits<ShapePair>(), "shared memory");
 
 struct TileArgs {
     const void *bias, *up_bias, *residual;
@@ -88,6 +95,7 @@ struct TileArgs {
     int rows, x_rows, N, n_k, groups;
     int feat_tiles;  // column tiles of out
     int box_rows;    // token rows of one TMA box
+    int stages;      // of the operand pipeline
     int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair); above 1 one tile a cluster
     int block;       // token tiles that run together through the feature tiles (L2 reuse of x and W)
     int act;
@@ -317,7 +325,8 @@ __global__ void __launch_bounds__(kThreads, S::kBlocks)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap umap,
                       const TileArgs a) {
     extern __shared__ uint8_t smem_raw[];
-    constexpr int kTok = S::kTok, kStages = S::kStages, kStage = S::kStage;
+    constexpr int kTok = S::kTok, kStage = S::kStage;
+    const uint32_t stages = (uint32_t)a.stages;
     constexpr bool PAIR = S::kPair;
     using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -328,8 +337,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-    float* staging = reinterpret_cast<float*>(base_ptr + kStages * kStage);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + 2 * S::kBuffers * kStaging);
+    float* staging = reinterpret_cast<float*>(base_ptr + stages * kStage);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + stages * kStage + 2 * S::kBuffers * kStaging);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
     int* g_off = reinterpret_cast<int*>(tmem_slot + 4);
     int* g_tiles = g_off + a.groups + 1;
@@ -427,7 +436,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 if (lane < 2) tma_load_3d<PAIR>(dst + lane * kHalfBytes, my_w, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
                 else if (!gather && lane - 2 < boxes) tma_load_2d<PAIR>(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, row0 + (lane - 2) * a.box_rows);
                 if (gather && lane < boxes) tma_gather4(dst + kWBytes + lane * 512, &xmap, full, k0, quad);
-                if (++s == kStages) { s = 0; ephase ^= 1; }
+                if (++s == stages) { s = 0; ephase ^= 1; }
             }
         }
         timed_out = __any_sync(0xffffffffu, timed_out);
@@ -460,7 +469,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                     tc_commit<PAIR>(bar(B_EMPTY + s));
                     ++s;
                     off += kStage >> 4;
-                    if (s == kStages) { s = 0; off = 0; phase ^= 1; }
+                    if (s == stages) { s = 0; off = 0; phase ^= 1; }
                 }
                 if (ok) tc_commit<PAIR>(bar(B_ACC_FULL + buf));
             }
@@ -773,44 +782,47 @@ bool rows_for_tma(const void* base, int64_t inner, int64_t rows, int64_t stride,
     return outer <= 1 || (outer_stride % 8 == 0 && outer_stride >= 8 && outer_stride < (1LL << 38));
 }
 
-// How many clusters of `size` blocks of a kernel the device holds at once (0: none); asked once per kernel, device and size.
-int resident_clusters(const void* kernel, int size, int threads, int smem, int dev, int sms) {
-    struct Known { const void* kernel; int size, threads, dev, clusters; };
+// How many clusters of `size` blocks of a kernel, one block an SM, the device holds at once (0: none); asked once per kernel,
+// device and size.
+int resident_clusters(const void* kernel, int size, int dev, int sms) {
+    struct Known { const void* kernel; int size, dev, clusters; };
     static std::mutex mu;
     static std::vector<Known> known;
     std::lock_guard<std::mutex> lock(mu);
     for (const Known& k : known)
-        if (k.kernel == kernel && k.size == size && k.threads == threads && k.dev == dev) return k.clusters;
+        if (k.kernel == kernel && k.size == size && k.dev == dev) return k.clusters;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)size; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(2 * sms / size * size)); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.gridDim = dim3((unsigned)(sms / size * size)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = kSmemPerBlock;
     cfg.attrs = &attr; cfg.numAttrs = 1;
     int clusters = 0;
     if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
     cudaGetLastError();  // a refusal only means "not available"
-    known.push_back({kernel, size, threads, dev, clusters});
+    clusters = std::max(0, std::min(clusters, sms / size));
+    known.push_back({kernel, size, dev, clusters});
     return clusters;
 }
 
 template <typename S, bool BF16>
-int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int dev, int sms, cudaStream_t stream) {
+int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared_sm, int dev, int sms, cudaStream_t stream) {
     auto kernel = linear_tcgen05_kernel<S, BF16>;
     const void* k = reinterpret_cast<const void*>(kernel);
-    const int rc = allow_shared_memory_once(k, S::smem(kMaxGroups));
+    const int rc = allow_shared_memory_once(k, kSmemPerBlock);
     if (rc != SFB_OK) return rc;
-    const int cluster = S::kPair ? 2 : a.split, threads = kThreads;
-    int resident = sms * S::kBlocks;
-    if (cluster > 1 && (resident = resident_clusters(k, cluster, threads, S::smem(kMaxGroups), dev, sms)) == 0)
+    a.stages = S::stages(shared_sm ? kSmemPerHalf : kSmemPerBlock, a.groups);
+    const int cluster = S::kPair ? 2 : a.split, smem = S::smem(a.stages, a.groups);
+    int resident = sms * (shared_sm ? 2 : 1);
+    if (cluster > 1 && (resident = resident_clusters(k, cluster, dev, sms)) == 0)
         return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)cluster; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)((a.split > 1 ? units : std::min<int64_t>(units, resident)) * cluster));
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)S::smem(a.groups);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
     SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], a));
@@ -819,27 +831,32 @@ int launch_tiles(const CUtensorMap* maps, const TileArgs& a, int64_t units, int 
 
 }  // namespace
 
-// Every candidate shape is priced in clocks: rounds of tiles on the busiest thread block x (its K steps x a step + a tile's
-// fixed cost).  A step takes the longer of its MMAs (2 clocks a token column) and its operands' way into shared memory, and no
-// less than the issuing thread's own chain.
+// Every candidate shape is priced in clocks: a start, then the longer of the weights' way from HBM (3400 bytes a clock) and the
+// rounds of tiles on the busiest SM x their K steps x a step.  A step takes the longest of its MMAs (2 clocks a token column),
+// its operands' way into shared memory (48 bytes a clock an SM; 64 where a cluster shares them), its part of the 2200 clocks
+// that an operand takes to arrive, and the row gathers (60 clocks for four rows).  Two blocks an SM share the first two.  A
+// split launches a cluster for every tile and exchanges sums at its end; the clusters that fit are fewer than the SMs suggest.
 LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
     LinearPlan best{};
     int64_t best_cost = -1;
-    const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows;
+    const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows, used = grouped ? std::min(groups, rows) : 1;
     // only the mean of the groups is known here: a group is taken to have two standard deviations of an even draw more
     const int64_t likely = grouped ? mean + (int64_t)(2 * std::sqrt((double)mean)) : rows;
+    const int64_t from_hbm = used * K * N * (gated ? 4 : 2) / 3400;
     auto consider = [&](int tokens, bool pair, int split, bool order) {
-        const int64_t token_tiles = (grouped ? std::min(groups, rows) : 1) * ceil_div(likely, (int64_t)tokens);
+        const int64_t tiles_a_group = ceil_div(likely, (int64_t)tokens), width = ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16;
         const int64_t feat_tiles = ceil_div(N, (int64_t)((gated ? kFeat / 2 : kFeat) * (pair ? 2 : 1)));
-        const int64_t width = std::min<int64_t>(tokens, ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16);
-        const int64_t bytes = kWBytes + width * (pair ? 64 : 128);
-        int64_t step = std::max<int64_t>({2 * width, bytes / (pair ? 64 : 48), 400});
-        if (indexed && !order) step = std::max(step, std::min(width, mean) / 4 * 62);
-        const int64_t fixed = 2500 + 20 * width + (split > 1 ? 3000 : 0);
-        const int64_t slots = std::max(1, sms * (tokens <= 64 ? 2 : 1) / (pair ? 2 : split));
-        int64_t cost = ceil_div(token_tiles * feat_tiles, slots) * (ceil_div(n_k, (int64_t)split) * step + fixed);
+        const int64_t tiles = used * tiles_a_group * feat_tiles, blocks = tiles * (pair ? 2 : split);
+        const int an_sm = tokens <= 64 && blocks > sms ? 2 : 1, stages = an_sm == 2 ? (tokens == 32 ? 4 : 3) : tokens == 32 ? 9 : tokens == 64 ? 7 : 5;
+        const int64_t slots = std::max<int64_t>(1, pair ? sms / 2 : split == 1 ? sms * an_sm : sms * an_sm * 86 / (100 * split));
+        const int64_t rounds = ceil_div(tiles, slots), bytes = kWBytes + width * (pair ? 64 : 128);
+        int64_t step = std::max<int64_t>(an_sm * std::max(2 * width, bytes / (pair ? 64 : 48)), 2200 / stages);
+        if (indexed && !order) step = std::max(step, an_sm * std::min(width, mean) / 4 * 62);
+        // an uneven last round costs bandwidth too, if less than its share
+        const int64_t hbm = rounds > 1 ? (from_hbm + from_hbm * rounds * slots / tiles) / 2 : from_hbm;
+        int64_t cost = 6000 + 15 * width + std::max(hbm, rounds * ceil_div(n_k, (int64_t)split) * step) + (split > 1 ? 3000 + 6000 * (rounds - 1) : 0);
         if (order) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
-        if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, feat_tiles}; }
+        if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, an_sm, feat_tiles}; }
     };
     for (int order = 0; order <= (indexed && ordered ? 1 : 0); ++order) {
         for (int tokens : {32, 64, 128})
@@ -904,7 +921,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     const bool bf16 = in.dtype == SFB_BF16;
     auto go = [&](auto shape) {
         using S = decltype(shape);
-        return bf16 ? launch_tiles<S, true>(maps, a, units, dev, sms, stream) : launch_tiles<S, false>(maps, a, units, dev, sms, stream);
+        return bf16 ? launch_tiles<S, true>(maps, a, units, plan.blocks_an_sm == 2, dev, sms, stream) : launch_tiles<S, false>(maps, a, units, plan.blocks_an_sm == 2, dev, sms, stream);
     };
     if (plan.pair) return go(ShapePair{});
     return plan.tokens == 32 ? go(Shape32{}) : plan.tokens == 64 ? go(Shape64{}) : go(Shape128{});
