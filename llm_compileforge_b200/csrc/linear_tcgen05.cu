@@ -9,9 +9,11 @@
 // thread block whatever the shape.
 //
 // Persistent thread blocks walk the tiles; accumulators are double-buffered in tensor memory (2 x kTok columns):
-//   warp 8      TMA producer: per 64-wide K step two boxes of 64 features, and the token rows as boxes of box_rows rows
-//               or, with a row index, as row gathers of four rows (about 60 clocks each, whatever they bring: right for the
-//               few rows an expert has in decode; for many a pass before this kernel lays the rows out in index order)
+//   warp 8      weights' producer: per 64-wide K step two TMA boxes of 64 features
+//   warp 10     rows' producer: boxes of box_rows token rows, or, with a row index, row gathers of four rows (about 60 clocks
+//               each, whatever they bring: right for the few rows an expert has in decode; for many a pass before this kernel
+//               lays the rows out in index order).  One warp for both was the bound of every shape: a wait that succeeds 80
+//               clocks, a box 53, 600 a K step with the rest, against 512 for its MMAs.
 //   warp 9      one thread issues tcgen05.mma kind::f16 (N = tokens, K 16, four per step); the weight operand is MN-major for
 //               [K, N] storage and K-major for [N, K], straight from 128-byte-swizzled shared memory
 //   warps 0-7   epilogue, two groups of four warps that take every other 16 tokens: through a transposing buffer in shared
@@ -43,7 +45,7 @@ constexpr int kFeat = 128, kStepK = 64, kChunk = 16;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
 constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]
-constexpr int kEpilogueWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr int kEpilogueWarps = 8, kWeightWarp = 8, kMmaWarp = 9, kRowWarp = 10, kThreads = 352;
 constexpr uint32_t kSpin = 1u << 21;
 constexpr int kMaxSplit = 8;
 
@@ -346,10 +348,10 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     auto leader_bar = [&](int i) { return PAIR ? peer_addr(bar(i), 0) : bar(i); };
 
-    if (warp == kTmaWarp) {  // one barrier a lane
+    if (warp == kWeightWarp) {  // one barrier a lane
         if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &wmap : lane == 1 ? &xmap : &umap) : "memory");
         for (int i = lane; i < B_COUNT; i += 32)
-            mbar_init(bar(i), i < B_ACC_EMPTY ? 1 : kEpilogueWarps * (PAIR ? 2 : 1));
+            mbar_init(bar(i), i < B_EMPTY ? 2 : i < B_ACC_EMPTY ? 1 : kEpilogueWarps * (PAIR ? 2 : 1));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -400,18 +402,39 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     auto own_rows = [&](const Tile& t, int r) { return PAIR ? max(0, min(half_of(t), t.rows - r * half_of(t))) : t.rows; };
     bool timed_out = false;
 
-    if (warp == kTmaWarp) {
-        // ============================ TMA producer ============================
-        // Lanes 0 and 1 load the weights, lane 2 + j token box j; with a row index lane j the j-th four rows.
+    if (warp == kWeightWarp) {
+        // ========================= weights' producer ==========================
+        if (lane == 0) {
+            const uint32_t bytes = (PAIR ? 2 : 1) * kWBytes;
+            const CUtensorMap* const second = a.gated ? &umap : &wmap;
+            const uint32_t full0 = leader_bar(B_FULL);
+            uint32_t s = 0, ephase = 1;
+            for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
+                const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
+                const int n0 = column0(tile), n1 = n0 + (a.gated ? 0 : 64);
+                for (int k = k_first; k < k_end; ++k) {
+                    if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
+                    if (!PAIR || rank == 0) mbar_expect_tx(bar(B_FULL + s), bytes);
+                    const uint32_t full = full0 + 8 * s, dst = base + s * kStage;
+                    const int k0 = k * kStepK;
+                    tma_load_3d<PAIR>(dst, &wmap, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
+                    tma_load_3d<PAIR>(dst + kHalfBytes, second, full, a.nk ? k0 : n1, a.nk ? n1 : k0, tile.group);
+                    if (++s == stages) { s = 0; ephase ^= 1; }
+                }
+            }
+        }
+    } else if (warp == kRowWarp) {
+        // =========================== rows' producer ===========================
+        // Lane j loads the j-th box, with a row index the j-th four rows.
+        const uint32_t full0 = leader_bar(B_FULL);
         uint32_t s = 0, ephase = 1;
         for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
             const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
-            const int n0 = column0(tile) + (a.gated ? 0 : lane * 64);  // lanes 0 and 1
-            const CUtensorMap* my_w = a.gated && lane == 1 ? &umap : &wmap;
             auto boxes_of = [&](int r) { return gather ? (tile.rows + 3) / 4 : (own_rows(tile, r) + a.box_rows - 1) / a.box_rows; };
             const int boxes = boxes_of(rank), all = PAIR ? boxes_of(0) + boxes_of(1) : boxes;
-            const uint32_t bytes = (PAIR ? 2 : 1) * kWBytes + all * (gather ? 4 : a.box_rows) * 128;
-            const int row0 = tile.row0 + (PAIR ? rank * half_of(tile) : 0);
+            const uint32_t bytes = all * (gather ? 4 : a.box_rows) * 128;
+            const int row = tile.row0 + (PAIR ? rank * half_of(tile) : 0) + lane * a.box_rows;
+            const uint32_t place = base + kWBytes + lane * (gather ? 512 : a.box_rows * 128);
             int4 quad = make_int4(0, 0, 0, 0);
             if (gather) {
                 int r[4];
@@ -428,14 +451,11 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
             for (int k = k_first; k < k_end; ++k) {
                 if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
-                const uint32_t dst = base + s * kStage;
                 if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), bytes);
-                __syncwarp();
-                const uint32_t full = leader_bar(B_FULL + s);
-                const int k0 = k * kStepK;
-                if (lane < 2) tma_load_3d<PAIR>(dst + lane * kHalfBytes, my_w, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
-                else if (!gather && lane - 2 < boxes) tma_load_2d<PAIR>(dst + kWBytes + (lane - 2) * a.box_rows * 128, &xmap, full, k0, row0 + (lane - 2) * a.box_rows);
-                if (gather && lane < boxes) tma_gather4(dst + kWBytes + lane * 512, &xmap, full, k0, quad);
+                if (lane < boxes) {
+                    if (gather) tma_gather4(place + s * kStage, &xmap, full0 + 8 * s, k * kStepK, quad);
+                    else tma_load_2d<PAIR>(place + s * kStage, &xmap, full0 + 8 * s, k * kStepK, row);
+                }
                 if (++s == stages) { s = 0; ephase ^= 1; }
             }
         }
@@ -892,8 +912,8 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     a.feat_tiles = (int)plan.feat_tiles; a.split = plan.split; a.act = in.act;
     a.gated = in.up != nullptr; a.nk = nk; a.out_f32 = in.out_dtype == SFB_F32;
     a.block = 8;
-    // one box where the rows fit one (in eights), boxes of 32 else: the last one of a group brings in at most 31 rows too many
-    a.box_rows = !in.offsets && in.rows <= 32 ? (int)(ceil_div(in.rows, (int64_t)8) * 8) : 32;
+    // rows of a box: all where they fit one (in eights); else 32, or 64 of a pair's 128, the last one bringing in some too many
+    a.box_rows = !in.offsets && in.rows <= 32 ? (int)(ceil_div(in.rows, (int64_t)8) * 8) : plan.pair ? 64 : 32;
     const bool order = plan.order;
     const void* x = order ? in.workspace : in.x;
     const int64_t x_rows = order ? in.rows : in.x_rows, x_row = order || x_rows == 1 ? ordered_stride : in.x_stride;
