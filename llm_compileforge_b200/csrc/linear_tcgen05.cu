@@ -67,10 +67,10 @@ struct Shape {
     static constexpr int kRows = PAIR ? TOK / 2 : TOK;  // token rows in one block's shared memory
     static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
     static constexpr int kBuffers = TOK == 32 ? 1 : 2;  // staging buffers of an epilogue group; one where it has one chunk a tile
-    static constexpr int kStage = kWBytes + kRows * 128;
-    static constexpr int smem(int stages, int groups) { return 1024 + stages * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
-    static constexpr int stages(int budget, int groups) {
-        const int n = (budget - smem(0, groups)) / kStage;
+    static constexpr int kStage = kWBytes + kRows * 128;  // of one K step
+    static constexpr int smem(int steps, int groups) { return 1024 + steps * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
+    static constexpr int stages(int budget, int groups, int sub) {  // of `sub` K steps each
+        const int n = (budget - smem(0, groups)) / (sub * kStage);
         return n < kMaxStages ? n : kMaxStages;
     }
 };
@@ -83,8 +83,8 @@ using ShapePair = Shape<256, 1, true>;
 constexpr int kSmemPerBlock = 232448, kSmemPerHalf = 233472 / 2 - 1024;  // of one block an SM, of each of two
 template <typename S>
 constexpr bool fits() {  // a pipeline at all, and room for a tile's sums in it
-    const int n = S::stages(S::kBlocks == 2 ? kSmemPerHalf : kSmemPerBlock, kMaxGroups);
-    return n >= 2 && S::kTok * kFeat * 4 <= n * S::kStage * (S::kPair ? 2 : 1);
+    const int one = S::stages(kSmemPerHalf, kMaxGroups, 1), two = S::stages(kSmemPerBlock, kMaxGroups, 2);
+    return (S::kBlocks == 1 || (one >= 2 && S::kTok * kFeat * 4 <= one * S::kStage)) && two >= 2 && (S::kPair || S::kTok * kFeat * 4 <= two * 2 * S::kStage);
 }
 static_assert(fits<Shape32>() && fits<Shape64>() && fits<Shape128>() && fits<ShapePair>(), "shared memory");
 
@@ -98,6 +98,7 @@ struct TileArgs {
     int feat_tiles;  // column tiles of out
     int box_rows;    // token rows of one TMA box
     int stages;      // of the operand pipeline
+    int sub;         // 64-wide K steps of a stage, behind one pair of barriers
     int split;       // thread blocks that share a tile's K steps (= cluster size, without kPair); above 1 one tile a cluster
     int block;       // token tiles that run together through the feature tiles (L2 reuse of x and W)
     int act;
@@ -328,7 +329,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                       const TileArgs a) {
     extern __shared__ uint8_t smem_raw[];
     constexpr int kTok = S::kTok, kStage = S::kStage;
-    const uint32_t stages = (uint32_t)a.stages;
+    const uint32_t stages = (uint32_t)a.stages, sub = (uint32_t)a.sub, stage_bytes = sub * kStage;
     constexpr bool PAIR = S::kPair;
     using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -339,8 +340,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-    float* staging = reinterpret_cast<float*>(base_ptr + stages * kStage);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + stages * kStage + 2 * S::kBuffers * kStaging);
+    float* staging = reinterpret_cast<float*>(base_ptr + stages * stage_bytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + stages * stage_bytes + 2 * S::kBuffers * kStaging);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
     int* g_off = reinterpret_cast<int*>(tmem_slot + 4);
     int* g_tiles = g_off + a.groups + 1;
@@ -412,13 +413,16 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
                 const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
                 const int n0 = column0(tile), n1 = n0 + (a.gated ? 0 : 64);
-                for (int k = k_first; k < k_end; ++k) {
+                for (int k = k_first; k < k_end; k += sub) {
                     if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
-                    if (!PAIR || rank == 0) mbar_expect_tx(bar(B_FULL + s), bytes);
-                    const uint32_t full = full0 + 8 * s, dst = base + s * kStage;
-                    const int k0 = k * kStepK;
-                    tma_load_3d<PAIR>(dst, &wmap, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
-                    tma_load_3d<PAIR>(dst + kHalfBytes, second, full, a.nk ? k0 : n1, a.nk ? n1 : k0, tile.group);
+                    const int end = min(k + (int)sub, k_end);
+                    if (!PAIR || rank == 0) mbar_expect_tx(bar(B_FULL + s), (end - k) * bytes);
+                    const uint32_t full = full0 + 8 * s;
+                    uint32_t dst = base + s * stage_bytes;
+                    for (int k0 = k * kStepK; k0 < end * kStepK; k0 += kStepK, dst += kStage) {
+                        tma_load_3d<PAIR>(dst, &wmap, full, a.nk ? k0 : n0, a.nk ? n0 : k0, tile.group);
+                        tma_load_3d<PAIR>(dst + kHalfBytes, second, full, a.nk ? k0 : n1, a.nk ? n1 : k0, tile.group);
+                    }
                     if (++s == stages) { s = 0; ephase ^= 1; }
                 }
             }
@@ -449,12 +453,14 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 }
                 quad = make_int4(r[0], r[1], r[2], r[3]);
             }
-            for (int k = k_first; k < k_end; ++k) {
+            for (int k = k_first; k < k_end; k += sub) {
                 if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
-                if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), bytes);
-                if (lane < boxes) {
-                    if (gather) tma_gather4(place + s * kStage, &xmap, full0 + 8 * s, k * kStepK, quad);
-                    else tma_load_2d<PAIR>(place + s * kStage, &xmap, full0 + 8 * s, k * kStepK, row);
+                const int end = min(k + (int)sub, k_end);
+                if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), (end - k) * bytes);
+                uint32_t dst = place + s * stage_bytes;
+                for (int k0 = k * kStepK; k0 < end * kStepK && lane < boxes; k0 += kStepK, dst += kStage) {
+                    if (gather) tma_gather4(dst, &xmap, full0 + 8 * s, k0, quad);
+                    else tma_load_2d<PAIR>(dst, &xmap, full0 + 8 * s, k0, row);
                 }
                 if (++s == stages) { s = 0; ephase ^= 1; }
             }
@@ -478,7 +484,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * kTok;
-                for (int k = k_first; k < k_end; ++k) {
+                for (int k = k_first; k < k_end; k += sub) {
                     ok = PAIR ? mbar_wait_cluster(bar(B_FULL + s), phase) : mbar_wait(bar(B_FULL + s), phase);
                     if (!ok) break;
                     tc_fence_after();
@@ -486,9 +492,16 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                     mma_ss<PAIR>(d, w_lo0 + off + w_step, hi, x_lo0 + off + 2, hi, idesc, 1);
                     mma_ss<PAIR>(d, w_lo0 + off + 2 * w_step, hi, x_lo0 + off + 4, hi, idesc, 1);
                     mma_ss<PAIR>(d, w_lo0 + off + 3 * w_step, hi, x_lo0 + off + 6, hi, idesc, 1);
+                    if (k + 1 < min(k + (int)sub, k_end)) {  // the stage's second K step
+                        const uint32_t o = off + (kStage >> 4);
+                        mma_ss<PAIR>(d, w_lo0 + o, hi, x_lo0 + o, hi, idesc, 1);
+                        mma_ss<PAIR>(d, w_lo0 + o + w_step, hi, x_lo0 + o + 2, hi, idesc, 1);
+                        mma_ss<PAIR>(d, w_lo0 + o + 2 * w_step, hi, x_lo0 + o + 4, hi, idesc, 1);
+                        mma_ss<PAIR>(d, w_lo0 + o + 3 * w_step, hi, x_lo0 + o + 6, hi, idesc, 1);
+                    }
                     tc_commit<PAIR>(bar(B_EMPTY + s));
                     ++s;
-                    off += kStage >> 4;
+                    off += stage_bytes >> 4;
                     if (s == stages) { s = 0; off = 0; phase ^= 1; }
                 }
                 if (ok) tc_commit<PAIR>(bar(B_ACC_FULL + buf));
@@ -831,8 +844,9 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
     const void* k = reinterpret_cast<const void*>(kernel);
     const int rc = allow_shared_memory_once(k, kSmemPerBlock);
     if (rc != SFB_OK) return rc;
-    a.stages = S::stages(shared_sm ? kSmemPerHalf : kSmemPerBlock, a.groups);
-    const int cluster = S::kPair ? 2 : a.split, smem = S::smem(a.stages, a.groups);
+    a.sub = shared_sm ? 1 : 2;
+    a.stages = S::stages(shared_sm ? kSmemPerHalf : kSmemPerBlock, a.groups, a.sub);
+    const int cluster = S::kPair ? 2 : a.split, smem = S::smem(a.stages * a.sub, a.groups);
     int resident = sms * (shared_sm ? 2 : 1);
     if (cluster > 1 && (resident = resident_clusters(k, cluster, dev, sms)) == 0)
         return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
