@@ -16,7 +16,7 @@
 //               clocks, a box 53, 600 a K step with the rest, against 512 for its MMAs.
 //   warp 9      one thread issues tcgen05.mma kind::f16 (N = tokens, K 16, four per step); the weight operand is MN-major for
 //               [K, N] storage and K-major for [N, K], straight from 128-byte-swizzled shared memory
-//   warps 0-7   epilogue, two groups of four warps that take every other 16 tokens: through a transposing buffer in shared
+//   warps 0-7   epilogue, two groups of four warps that take every other 16 or 32 tokens: through a transposing buffer in shared
 //               memory, so that rows of out and residual move as 8 bytes a lane; bias, activation, gate, residual in fp32,
 //               one rounding
 // Many rows a group (kPair): a cluster of two thread blocks owns 256 features x 256 tokens with cta_group::2 MMAs (M 256): each
@@ -41,10 +41,9 @@
 namespace sfb {
 namespace {
 
-constexpr int kFeat = 128, kStepK = 64, kChunk = 16;
+constexpr int kFeat = 128, kStepK = 64;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
-constexpr int kStaging = kChunk * kFeat * 4;     // fp32 [16 tokens][128 features]
 constexpr int kEpilogueWarps = 8, kWeightWarp = 8, kMmaWarp = 9, kRowWarp = 10, kThreads = 352;
 constexpr uint32_t kSpin = 1u << 21;
 constexpr int kMaxSplit = 8;
@@ -66,7 +65,10 @@ struct Shape {
     static constexpr bool kPair = PAIR;
     static constexpr int kRows = PAIR ? TOK / 2 : TOK;  // token rows in one block's shared memory
     static constexpr int kRound = PAIR ? 32 : 16;       // what the MMA's N is a multiple of
-    static constexpr int kBuffers = TOK == 32 ? 1 : 2;  // staging buffers of an epilogue group; one where it has one chunk a tile
+    // The epilogue takes this many tokens at a time: 32 where the registers allow it; at 16 a 256-token tile took 860 clocks each
+    static constexpr int kChunk = TOK >= 128 ? 32 : 16;
+    static constexpr int kStaging = kChunk * kFeat * 4;  // fp32 [chunk][128 features]
+    static constexpr int kBuffers = TOK == 64 ? 2 : 1;   // of an epilogue group
     static constexpr int kStage = kWBytes + kRows * 128;  // of one K step
     static constexpr int smem(int steps, int groups) { return 1024 + steps * kStage + 2 * kBuffers * kStaging + B_COUNT * 8 + 16 + 2 * (groups + 1) * 4; }
     static constexpr int stages(int budget, int groups, int sub) {  // of `sub` K steps each
@@ -234,17 +236,24 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi,
             ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
             : "memory");
 }
-// Sixteen columns of this lane's row, waited for in the same statement: between a load and its wait nothing may touch the
-// registers, and across two statements the compiler could.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+// N columns of this lane's row, waited for in the same statement: between a load and its wait nothing may touch the registers,
+// and across two statements the compiler could.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
+    static_assert(N == 16 || N == 32, "columns");
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        " tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
+    if constexpr (N == 16)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr)
+            : "memory");
+    else
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(taddr)
+            : "memory");
 }
 // Shared-memory matrix descriptor words (sm_100 format): start address and leading byte offset in 16-byte units; stride byte
 // offset, version 1, 128-byte swizzle.
@@ -341,7 +350,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
     float* staging = reinterpret_cast<float*>(base_ptr + stages * stage_bytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + stages * stage_bytes + 2 * S::kBuffers * kStaging);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + stages * stage_bytes + 2 * S::kBuffers * S::kStaging);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
     int* g_off = reinterpret_cast<int*>(tmem_slot + 4);
     int* g_tiles = g_off + a.groups + 1;
@@ -512,7 +521,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         // ============================== epilogue ==============================
         const int group = warp >> 2, w4 = warp & 3;  // this group takes chunks group, group + 2, ..
         const int sync_id = 1 + group;
-        float* const stage0 = staging + S::kBuffers * group * (kStaging / 4);
+        constexpr int kChunk = S::kChunk, kStaged = S::kStaging / 4;
+        float* const stage0 = staging + S::kBuffers * group * kStaged;
         bool ok = true, gone = false;  // a warp whose wait ran out; its group then leaves together, at the next tile
         int it = 0, used = 0;          // chunks that this group has staged
         const int cols = a.gated ? 2 : 4;  // columns of out that a lane writes for a token
@@ -559,9 +569,13 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
         };
 
-        // A tile of 16-bit rows in whole pieces, the usual case: no branch between the loads of a chunk, and the next chunk's
-        // residual on its way while this one is worked on.  (With the choices made value by value a chunk
-        // took 1500 clocks, with a residual 5500.)
+        // Before chunk c is staged: whoever still reads the buffer's last one must be done.  With two buffers that follows from the
+        // barrier of the chunk between, with one chunk a tile from the next tile's.
+        auto buffer_free = [&](int c) {
+            if (S::kBuffers == 1 && kTok > 2 * kChunk && c != group) group_sync(sync_id);
+        };
+        // A tile of 16-bit rows in whole pieces, the usual case: no branch between the loads of a chunk, the residual on its way
+        // to L2 while the MMAs run.  (With the choices made value by value 16 tokens took 1500 clocks, with a residual 5500.)
         auto whole_pieces = [&](auto gated, auto with_residual) {
             constexpr bool GATED = decltype(gated)::value, RES = decltype(with_residual)::value;
             constexpr int kEach = kChunk / 4;
@@ -570,26 +584,33 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             const int64_t row0 = tile.row0 + group * kChunk + w4;
             T* out = static_cast<T*>(a.out) + row0 * a.out_stride + n;
             const T* res = RES ? static_cast<const T*>(a.residual) + row0 * a.res_stride + n : nullptr;
-            Word r[kEach];
-            auto load_residual = [&](int left) {
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    r[i] = Word{};
-                    if (in && w4 + 4 * i < left) r[i] = *reinterpret_cast<const Word*>(res + 4 * i * a.res_stride);
-                }
-                res += 2 * kChunk * a.res_stride;
-            };
-            if constexpr (RES) load_residual(tile.rows - group * kChunk);
+            if constexpr (RES) {
+                // 16 lanes cover a row's 128 bytes of pieces: one of them asks for the line
+                for (int m = 4 * group + w4; m < tile.rows; m += 8)
+                    if (in && (lane & 15) == 0)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const T*>(a.residual) + (tile.row0 + m) * a.res_stride + n));
+            }
             if (!wait_accumulator()) return;
             for (int c = group; c < chunks; c += 2, ++used) {
-                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * (kStaging / 4) : 0);
-                float v[kChunk];
-                tmem_ld16(acc + c * kChunk, v);
-                if (c + 2 >= chunks) release();
+                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * kStaged : 0);
+                const int left = tile.rows - c * kChunk;
+                Word r[RES ? kEach : 1];
+                if constexpr (RES) {
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
-                // one barrier a chunk: a buffer is written again two chunks on, after the next chunk's barrier (with one chunk a
-                // tile: after the next tile's)
+                    for (int i = 0; i < kEach; ++i) {
+                        r[i] = Word{};
+                        if (in && w4 + 4 * i < left) r[i] = *reinterpret_cast<const Word*>(res + 4 * i * a.res_stride);
+                    }
+                    res += 2 * kChunk * a.res_stride;
+                }
+                {
+                    float v[kChunk];
+                    tmem_ld<kChunk>(acc + c * kChunk, v);
+                    if (c + 2 >= chunks) release();
+                    buffer_free(c);
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
+                }
                 group_sync(sync_id);
                 float q[kEach][4];
 #pragma unroll
@@ -614,9 +635,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                             q[i][0] += f.x; q[i][1] += f.y; q[i][2] += g.x; q[i][3] += g.y;
                         }
                     }
-                    load_residual(tile.rows - (c + 2) * kChunk);
                 }
-                const int left = tile.rows - c * kChunk;
 #pragma unroll
                 for (int i = 0; i < kEach; ++i)
                     if (in && w4 + 4 * i < left) {
@@ -668,10 +687,11 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             if (!wait_accumulator()) return;
             for (int c = group; c < chunks; c += 2, ++used) {
                 const int left = tile.rows - c * kChunk;
-                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * (kStaging / 4) : 0);
+                float* stage = stage0 + (S::kBuffers == 2 ? (used & 1) * kStaged : 0);
                 float v[kChunk];
-                tmem_ld16(acc + c * kChunk, v);
+                tmem_ld<kChunk>(acc + c * kChunk, v);
                 if (c + 2 >= chunks) release();
+                buffer_free(c);
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) stage[i * kFeat + w4 * 32 + lane] = v[i];
                 group_sync(sync_id);
@@ -689,7 +709,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             float* sums = reinterpret_cast<float*>(base_ptr);  // all MMAs are done: the operands' room is free
             for (int c = group; there && c < chunks; c += 2) {
                 float v[kChunk];
-                tmem_ld16(acc + c * kChunk, v);
+                tmem_ld<kChunk>(acc + c * kChunk, v);
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i)
                     if (c * kChunk + i < tile.rows) sums[(c * kChunk + i) * kFeat + w4 * 32 + lane] = v[i];
@@ -865,11 +885,12 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
 
 }  // namespace
 
-// Every candidate shape is priced in clocks: a start, then the longer of the weights' way from HBM (3400 bytes a clock) and the
-// rounds of tiles on the busiest SM x their K steps x a step.  A step takes the longest of its MMAs (2 clocks a token column),
-// its operands' way into shared memory (48 bytes a clock an SM; 64 where a cluster shares them), its part of the 2200 clocks
-// that an operand takes to arrive, and the row gathers (60 clocks for four rows).  Two blocks an SM share the first two.  A
-// split launches a cluster for every tile and exchanges sums at its end; the clusters that fit are fewer than the SMs suggest.
+// Every candidate shape is priced in clocks: a start and the last tile's epilogue, and between them the longer of the weights'
+// way from HBM (3400 bytes a clock) and the rounds of tiles on the busiest SM x their K steps x a step.  A step takes the longest
+// of its MMAs (2 clocks a token column), its operands' way into shared memory (72 bytes a clock an SM), the issuing thread's
+// chain (380 clocks with two steps a stage, 600 with one) and the row gathers (62 clocks for four rows); two blocks an SM share
+// the first two.  A split launches a cluster for every tile and exchanges sums at its end; how many clusters run at once goes
+// by the smallest of the eight groups of SMs that a cluster must lie in.
 LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
     LinearPlan best{};
     int64_t best_cost = -1;
@@ -881,14 +902,14 @@ LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool 
         const int64_t tiles_a_group = ceil_div(likely, (int64_t)tokens), width = ceil_div(ceil_div(mean, ceil_div(mean, (int64_t)tokens)), (int64_t)16) * 16;
         const int64_t feat_tiles = ceil_div(N, (int64_t)((gated ? kFeat / 2 : kFeat) * (pair ? 2 : 1)));
         const int64_t tiles = used * tiles_a_group * feat_tiles, blocks = tiles * (pair ? 2 : split);
-        const int an_sm = tokens <= 64 && blocks > sms ? 2 : 1, stages = an_sm == 2 ? (tokens == 32 ? 4 : 3) : tokens == 32 ? 9 : tokens == 64 ? 7 : 5;
-        const int64_t slots = std::max<int64_t>(1, pair ? sms / 2 : split == 1 ? sms * an_sm : sms * an_sm * 86 / (100 * split));
+        const int an_sm = tokens <= 64 && blocks > sms ? 2 : 1;
+        const int64_t slots = std::max<int64_t>(1, pair ? sms / 2 : split == 1 ? sms * an_sm : 8 * (std::max(1, sms / 8 - 2) * an_sm / split));
         const int64_t rounds = ceil_div(tiles, slots), bytes = kWBytes + width * (pair ? 64 : 128);
-        int64_t step = std::max<int64_t>(an_sm * std::max(2 * width, bytes / (pair ? 64 : 48)), 2200 / stages);
+        int64_t step = std::max<int64_t>(an_sm * std::max(2 * width, bytes / 72), an_sm == 2 ? 600 : 380);
         if (indexed && !order) step = std::max(step, an_sm * std::min(width, mean) / 4 * 62);
         // an uneven last round costs bandwidth too, if less than its share
         const int64_t hbm = rounds > 1 ? (from_hbm + from_hbm * rounds * slots / tiles) / 2 : from_hbm;
-        int64_t cost = 6000 + 15 * width + std::max(hbm, rounds * ceil_div(n_k, (int64_t)split) * step) + (split > 1 ? 3000 + 6000 * (rounds - 1) : 0);
+        int64_t cost = 6000 + 25 * width + std::max(hbm, rounds * ceil_div(n_k, (int64_t)split) * step) + (split > 1 ? 3000 + 6000 * (rounds - 1) : 0);
         if (order) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
         if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, an_sm, feat_tiles}; }
     };
