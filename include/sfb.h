@@ -491,6 +491,11 @@ SFB_API int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, cons
                                int weight_layout, int dtype, int out_dtype, int activation, int32_t* status, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Host arithmetic only (no device call): the tile shape that sfb_fused_linear (groups 0) or sfb_grouped_linear runs for 16-bit
+ * operands that the tensor cores take, on a device with `sms` SMs.  plan6 = {token rows of a tile, cluster of two on a tile
+ * (0/1), thread blocks that share a tile's K, rows put in order first (0/1), thread blocks an SM, tiles across the columns}. */
+SFB_API int sfb_linear_plan(int64_t rows, int64_t K, int64_t N, int64_t groups, int gated, int indexed, int has_workspace, int sms, int32_t* plan6);
+
 /* The top_k experts of every token and the assignments sorted by expert.
  *   logits [T, E] (F32 | BF16 | F16), E <= 1024; top_k <= min(E, 32)
  *   expert_ids int32, weights float32, positions int32, each [T, top_k] contiguous;

@@ -199,6 +199,8 @@ def _feed_forward_protos(lib: ctypes.CDLL) -> None:
     lib.sfb_grouped_linear.argtypes = [t] * 8 + [c_int] * 4 + [c_void_p, c_void_p, c_int64, c_void_p]
     lib.sfb_grouped_linear_workspace_bytes.restype = c_int64
     lib.sfb_grouped_linear_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
+    lib.sfb_linear_plan.restype = c_int
+    lib.sfb_linear_plan.argtypes = [c_int64] * 4 + [c_int] * 4 + [POINTER(c_int32)]
     lib.sfb_moe_route_workspace_bytes.restype = c_int64
     lib.sfb_moe_route_workspace_bytes.argtypes = [c_int64, c_int64]
     lib.sfb_moe_route.restype = c_int

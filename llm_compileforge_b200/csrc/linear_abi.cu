@@ -136,6 +136,13 @@ int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTen
     return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
 
+int sfb_linear_plan(int64_t rows, int64_t K, int64_t N, int64_t groups, int gated, int indexed, int has_workspace, int sms, int32_t* plan6) {
+    if (rows < 1 || K < 1 || N < 1 || groups < 0 || groups > kMaxGroups || sms < 1 || !plan6) return fail(SFB_ERR_INVALID_ARG, "linear_plan: bad argument");
+    const LinearPlan p = plan_linear(rows, K, N, groups ? groups : 1, groups > 0, gated != 0, groups > 0 && indexed, has_workspace != 0, sms);
+    plan6[0] = p.tokens; plan6[1] = p.pair; plan6[2] = p.split; plan6[3] = p.order; plan6[4] = p.blocks_an_sm; plan6[5] = (int32_t)p.feat_tiles;
+    return SFB_OK;
+}
+
 int64_t sfb_moe_route_workspace_bytes(int64_t tokens, int64_t experts) {
     if (tokens < 0 || experts < 0) return SFB_ERR_INVALID_ARG;
     const int64_t blocks = ceil_div(tokens, (int64_t)kRouteTokens);

@@ -45,7 +45,7 @@ constexpr int kFeat = 128, kStepK = 64;
 constexpr int kWBytes = kFeat * kStepK * 2;      // a K step's weights: two boxes of 64 features
 constexpr int kHalfBytes = kWBytes / 2;
 constexpr int kEpilogueWarps = 8, kWeightWarp = 8, kMmaWarp = 9, kRowWarp = 10, kThreads = 352;
-constexpr uint32_t kSpin = 1u << 21;
+constexpr uint64_t kWaitNanoseconds = 2000000000;  // no wait of a kernel that takes milliseconds comes near it
 constexpr int kMaxSplit = 8;
 
 constexpr int kMaxStages = 9;
@@ -117,29 +117,31 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpin; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
+__device__ __forceinline__ uint64_t nanoseconds() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
 }
-// The same for barriers on which other blocks of the cluster arrive: what they wrote before is visible after.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpin; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
+// CLUSTER: for barriers on which other blocks of the cluster arrive; what they wrote before is visible after.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    if constexpr (CLUSTER)
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+// Waits kWaitNanoseconds at most.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_try<CLUSTER>(bar, parity)) return true;
+    const uint64_t begun = nanoseconds();
+    do {
+        if (mbar_try<CLUSTER>(bar, parity)) return true;
+    } while (nanoseconds() - begun < kWaitNanoseconds);
     return false;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -494,7 +496,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 tc_fence_after();
                 const uint32_t d = tmem + buf * kTok;
                 for (int k = k_first; k < k_end; k += sub) {
-                    ok = PAIR ? mbar_wait_cluster(bar(B_FULL + s), phase) : mbar_wait(bar(B_FULL + s), phase);
+                    ok = mbar_wait<PAIR>(bar(B_FULL + s), phase);
                     if (!ok) break;
                     tc_fence_after();
                     mma_ss<PAIR>(d, w_lo0 + off, hi, x_lo0 + off, hi, idesc, k > k_first);
@@ -542,7 +544,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
         };
         auto wait_accumulator = [&] {
-            if (ok) ok = PAIR ? mbar_wait_cluster(bar(B_ACC_FULL + buf), (it >> 1) & 1) : mbar_wait(bar(B_ACC_FULL + buf), (it >> 1) & 1);
+            if (ok) ok = mbar_wait<PAIR>(bar(B_ACC_FULL + buf), (it >> 1) & 1);
             gone = group_any(sync_id, !ok);
             if (gone) return ok = false;
             tc_fence_after();
@@ -887,7 +889,7 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
 
 // Every candidate shape is priced in clocks: a start and the last tile's epilogue, and between them the longer of the weights'
 // way from HBM (3400 bytes a clock) and the rounds of tiles on the busiest SM x their K steps x a step.  A step takes the longest
-// of its MMAs (2 clocks a token column), its operands' way into shared memory (72 bytes a clock an SM), the issuing thread's
+// of its MMAs (2 clocks a token column, with what lies between them 2.3 for a pair), its operands' way into shared memory (72 bytes a clock an SM), the issuing thread's
 // chain (380 clocks with two steps a stage, 600 with one) and the row gathers (62 clocks for four rows); two blocks an SM share
 // the first two.  A split launches a cluster for every tile and exchanges sums at its end; how many clusters run at once goes
 // by the smallest of the eight groups of SMs that a cluster must lie in.
@@ -905,11 +907,13 @@ LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool 
         const int an_sm = tokens <= 64 && blocks > sms ? 2 : 1;
         const int64_t slots = std::max<int64_t>(1, pair ? sms / 2 : split == 1 ? sms * an_sm : 8 * (std::max(1, sms / 8 - 2) * an_sm / split));
         const int64_t rounds = ceil_div(tiles, slots), bytes = kWBytes + width * (pair ? 64 : 128);
-        int64_t step = std::max<int64_t>(an_sm * std::max(2 * width, bytes / 72), an_sm == 2 ? 600 : 380);
+        int64_t step = std::max<int64_t>(an_sm * std::max(pair ? 23 * width / 10 : 2 * width, bytes / 72), an_sm == 2 ? 600 : 380);
         if (indexed && !order) step = std::max(step, an_sm * std::min(width, mean) / 4 * 62);
         // an uneven last round costs bandwidth too, if less than its share
-        const int64_t hbm = rounds > 1 ? (from_hbm + from_hbm * rounds * slots / tiles) / 2 : from_hbm;
-        int64_t cost = 6000 + 25 * width + std::max(hbm, rounds * ceil_div(n_k, (int64_t)split) * step) + (split > 1 ? 3000 + 6000 * (rounds - 1) : 0);
+        const int64_t hbm = rounds > 1 ? (from_hbm + from_hbm * rounds * slots / tiles) / 2 : from_hbm, on_sm = rounds * ceil_div(n_k, (int64_t)split) * step;
+        // the two overlap, but not wholly
+        int64_t cost = 6000 + 25 * width + std::max(hbm, on_sm) + std::min(hbm, on_sm) / 4 + (an_sm - 1) * 1500;
+        if (split > 1) cost += 3000 + 300 * split + 6000 * (rounds - 1);
         if (order) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
         if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, an_sm, feat_tiles}; }
     };

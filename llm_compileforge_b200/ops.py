@@ -603,6 +603,17 @@ def grouped_linear_workspace_bytes(rows: int, k: int, groups: int, indexed: bool
     return int(n)
 
 
+def linear_plan(rows: int, k: int, n: int, *, groups: int = 0, gated: bool = False, indexed: bool = False, has_workspace: bool = True,
+                sms: int = 148) -> dict:
+    """The tile shape :func:`fused_linear` (``groups=0``) or :func:`grouped_linear` runs for 16-bit operands that the tensor cores
+    take (host arithmetic, no device needed)."""
+    import ctypes
+
+    out = (ctypes.c_int32 * 6)()
+    check(_lib.load().sfb_linear_plan(int(rows), int(k), int(n), int(groups), int(bool(gated)), int(bool(indexed)), int(bool(has_workspace)), int(sms), out))
+    return dict(zip(("tokens", "pair", "split", "order", "blocks_an_sm", "feature_tiles"), (int(v) for v in out)))
+
+
 class MoeRouting(NamedTuple):
     """What :func:`moe_route` returns; assignment ``(t, j)`` is row ``positions[t, j]`` of the order sorted by expert."""
 
