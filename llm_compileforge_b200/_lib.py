@@ -249,14 +249,19 @@ def packed(t: torch.Tensor | None, what: str, index: int):
     count; the tensor must live on CUDA device ``index``."""
     if t is None:
         return None
-    if t.get_device() != index or index < 0:  # -1: not a CUDA tensor
+    if index < 0 or t.get_device() != index:  # -1: not a CUDA tensor
         raise ValueError(f"{what} must live on {f'cuda:{index}' if index >= 0 else 'a CUDA device'} (libsfb has no CPU path), got {t.device}")
     shape = t.shape
     rank = len(shape)
-    if not 1 <= rank <= 4:
+    if not 0 < rank < 5:
         raise ValueError(f"{what}: rank {rank} outside 1..4")
     p = t.data_ptr()
-    return _PACK[rank](SFB_DEVICE_CUDA, rank, t.element_size(), 0, p, p, 0, *shape, *t.stride())
+    return _PACK[rank](2, rank, t.itemsize, 0, p, p, 0, *shape, *t.stride())  # 2: SFB_DEVICE_CUDA
+
+
+def packed_rows(p: int, *shape: int):
+    """Descriptor of a contiguous array of 4-byte values at device address ``p`` (rank 1 or 2)."""
+    return _PACK[1](2, 1, 4, 0, p, p, 0, shape[0], 1) if len(shape) == 1 else _PACK[2](2, 2, 4, 0, p, p, 0, *shape, shape[1], 1)
 
 
 def check(status: int) -> None:

@@ -893,7 +893,7 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
 // chain (380 clocks with two steps a stage, 600 with one) and the row gathers (62 clocks for four rows); two blocks an SM share
 // the first two.  A split launches a cluster for every tile and exchanges sums at its end; how many clusters run at once goes
 // by the smallest of the eight groups of SMs that a cluster must lie in.
-LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
+static LinearPlan price_shapes(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
     LinearPlan best{};
     int64_t best_cost = -1;
     const int64_t n_k = ceil_div(K, (int64_t)kStepK), mean = grouped ? ceil_div(rows, groups) : rows, used = grouped ? std::min(groups, rows) : 1;
@@ -923,6 +923,18 @@ LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool 
         if (!indexed || order) consider(256, true, 1, order);
     }
     return best;
+}
+
+// Pricing takes two microseconds of host time and a program calls with the same sizes again and again: each thread keeps the
+// shapes of the last sizes it met.
+LinearPlan plan_linear(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {
+    struct Priced { int64_t rows, K, N, groups; int flags, sms; LinearPlan plan; };
+    thread_local Priced known[64] = {};
+    const int flags = 16 | grouped | gated << 1 | indexed << 2 | ordered << 3;
+    Priced& p = known[(uint64_t)(rows * 31 + K * 17 + N * 7 + groups * 3 + flags) * 0x9e3779b97f4a7c15ULL >> 58];
+    if (p.rows != rows || p.K != K || p.N != N || p.groups != groups || p.flags != flags || p.sms != sms)
+        p = {rows, K, N, groups, flags, sms, price_shapes(rows, K, N, groups, grouped, gated, indexed, ordered, sms)};
+    return p.plan;
 }
 
 int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {

@@ -8,12 +8,13 @@ dict-based signatures of the reference's ``kernels`` package are in
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import call_on, check, current_stream, desc, dtype_code, packed
+from ._lib import call_on, check, current_stream, desc, dtype_code, packed, packed_rows
 
 BLOCK_SIZE = 16
 
@@ -459,10 +460,10 @@ ACTIVATIONS = {"none": _lib.SFB_ACT_NONE, "silu": _lib.SFB_ACT_SILU, "gelu": _li
                "relu": _lib.SFB_ACT_RELU}
 
 
-def _same_type(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
+def _same_type(what: str, dtype: torch.dtype, names: str, *tensors: torch.Tensor | None) -> None:
+    for i, t in enumerate(tensors):
         if t is not None and t.dtype is not dtype:
-            raise ValueError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+            raise ValueError(f"{what}: {names.split()[i]} is {t.dtype}, expected {dtype}")
 
 
 def _matrix(what: str, w: torch.Tensor, like: int | None = None) -> tuple[torch.Tensor, int]:
@@ -509,7 +510,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     k, n = ws
     act = _activation("fused_linear", activation)
     odt = out.dtype if out is not None else out_dtype or dtype
-    _same_type("fused_linear", dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
+    _same_type("fused_linear", dtype, "weight bias up_weight up_bias", weight, bias, up_weight, up_bias)
     if k == 0:
         raise ValueError("fused_linear: K is zero")
     flat = len(xs) == 2
@@ -574,8 +575,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     e, k, n = ws
     act = _activation("grouped_linear", activation)
     odt = out.dtype if out is not None else out_dtype or dtype
-    _same_type("grouped_linear", dtype, weight=weight, bias=bias, up_weight=up_weight, up_bias=up_bias)
-    _same_type("grouped_linear", torch.int32, group_offsets=group_offsets, row_index=row_index)
+    _same_type("grouped_linear", dtype, "weight bias up_weight up_bias", weight, bias, up_weight, up_bias)
+    _same_type("grouped_linear", torch.int32, "group_offsets row_index", group_offsets, row_index)
     if x.stride(1) != 1 and k > 1:
         x = x.contiguous()
     w, layout = _matrix("grouped_linear", weight)
@@ -596,6 +597,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     return out
 
 
+@lru_cache(maxsize=1024)
 def grouped_linear_workspace_bytes(rows: int, k: int, groups: int, indexed: bool = True) -> int:
     n = _lib.load().sfb_grouped_linear_workspace_bytes(int(rows), int(k), int(groups), int(bool(indexed)))
     if n < 0:
@@ -637,17 +639,19 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, wor
     (t, e), k, dev = ls, int(top_k), logits.get_device()
     if k < 1 or k > min(e, 32):
         raise ValueError(f"moe_route: top_k {k} outside 1 .. min(experts, 32)")
-    ids, positions = logits.new_empty((2, t, k), dtype=torch.int32).unbind(0)
-    weights = logits.new_empty((t, k), dtype=torch.float32)
-    rows, offsets = logits.new_empty(t * k, dtype=torch.int32), logits.new_empty(e + 1, dtype=torch.int32)
+    results = logits.new_empty((4, t, k), dtype=torch.int32)  # one allocation for the four of that size
+    offsets = logits.new_empty(e + 1, dtype=torch.int32)
     need = moe_route_workspace_bytes(t, e) if workspace is None else 0
     workspace, ws_ptr, ws_bytes = _workspace("moe_route", workspace, need, logits)
-    call_on(dev, _lib.load().sfb_moe_route, packed(logits, "logits", dev), packed(ids, "expert_ids", dev), packed(weights, "weights", dev),
-            packed(offsets, "group_offsets", dev), packed(rows, "token_rows", dev), packed(positions, "positions", dev), dtype_code(logits.dtype),
+    p, each = results.data_ptr(), 4 * t * k
+    call_on(dev, _lib.load().sfb_moe_route, packed(logits, "logits", dev), packed_rows(p, t, k), packed_rows(p + each, t, k),
+            packed(offsets, "group_offsets", dev), packed_rows(p + 2 * each, t * k), packed_rows(p + 3 * each, t, k), dtype_code(logits.dtype),
             1 if renormalize else 0, ws_ptr, ws_bytes)
-    return MoeRouting(ids, weights, offsets, rows, positions)
+    ids, weights, rows, positions = results.unbind(0)
+    return MoeRouting(ids, weights.view(torch.float32), offsets, rows.view(-1), positions)
 
 
+@lru_cache(maxsize=1024)
 def moe_route_workspace_bytes(tokens: int, experts: int) -> int:
     n = _lib.load().sfb_moe_route_workspace_bytes(int(tokens), int(experts))
     if n < 0:
@@ -665,7 +669,7 @@ def moe_combine(y: torch.Tensor, positions: torch.Tensor, weights: torch.Tensor,
         raise ValueError(f"moe_combine: y [R, H], positions and weights [T, k], got {tuple(ys)}, {tuple(ps)}, {tuple(weights.shape)}")
     if positions.dtype is not torch.int32 or weights.dtype is not torch.float32:
         raise ValueError(f"moe_combine: positions must be int32 and weights float32, got {positions.dtype} and {weights.dtype}")
-    _same_type("moe_combine", dtype, residual=residual, out=out)
+    _same_type("moe_combine", dtype, "residual out", residual, out)
     shape = (ps[0], ys[1])
     for name, t in (("out", out), ("residual", residual)):
         if t is not None and t.shape != shape:
