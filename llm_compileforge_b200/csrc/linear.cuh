@@ -2,6 +2,8 @@
 // kernels share.
 #pragma once
 
+#include <utility>
+
 #include "sfb_common.cuh"
 
 namespace sfb {
@@ -69,6 +71,27 @@ struct CombineArgs {
 int launch_moe_combine(const CombineArgs& a, cudaStream_t stream);
 
 #ifdef __CUDACC__
+// These kernels follow one another (router, product, product, sum), so each is launched before the one before it has ended
+// (programmatic dependent launch): its blocks start where that one's have left, set themselves up and wait here.  Every thread
+// that reads or writes global memory passes wait_for_previous first; let_next_start comes when a block holds all that it will
+// ask the SM for, so a waiting successor cannot keep anything from it.  A kernel that does not take part ends before its
+// successor starts.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int smem, unsigned cluster, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster; attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = stream;
+    cfg.attrs = attrs; cfg.numAttrs = cluster > 1 ? 2 : 1;
+    SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+    return SFB_OK;
+}
+
 // Group offsets come from the device and are not trusted: each is clamped to [0, rows], and one below an offset before it
 // counts as that one.  Groups then never overlap or leave the rows, whatever the array holds.
 __device__ __forceinline__ int group_offset(int raw, int before, int rows) { return max(before, min(raw, rows)); }

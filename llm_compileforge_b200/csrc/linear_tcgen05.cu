@@ -368,6 +368,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == kMmaWarp) tmem_alloc<PAIR>(smem_u32(tmem_slot), 2 * kTok);
+    wait_for_previous();
     if (warp == 0) {  // the groups' rows, and the running number of token tiles
         int before = 0, top = a.offsets ? group_offset(a.offsets[0], 0, a.rows) : 0;
         bool bad = a.offsets && top != a.offsets[0];
@@ -400,6 +401,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
     tc_fence_before();
     __syncthreads();
+    let_next_start();
     if constexpr (PAIR) cluster_sync();  // the other block's barriers exist before anything is sent to them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
@@ -777,6 +779,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
 __global__ void __launch_bounds__(256) order_rows_kernel(const uint16_t* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ row_index,
                                                          const int32_t* __restrict__ offsets, int groups, int rows, int x_rows, int K,
                                                          uint16_t* __restrict__ ordered, int64_t ordered_stride, int* status) {
+    let_next_start();
+    wait_for_previous();
     int first = group_offset(offsets[0], 0, rows), end = first;
     for (int e = threadIdx.x; e < groups; e += 256) end = group_offset(offsets[e + 1], end, rows);
     __shared__ int ends[256];
@@ -872,17 +876,8 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
     int resident = sms * (shared_sm ? 2 : 1);
     if (cluster > 1 && (resident = resident_clusters(k, cluster, dev, sms)) == 0)
         return fail(SFB_ERR_CUDA, "linear: the device holds no cluster of %d thread blocks", cluster);
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)cluster; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)((a.split > 1 ? units : std::min<int64_t>(units, resident)) * cluster));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = stream;
-    cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
-    SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], a));
-    return SFB_OK;
+    const unsigned grid = (unsigned)((a.split > 1 ? units : std::min<int64_t>(units, resident)) * cluster);
+    return launch_after(kernel, grid, kThreads, smem, (unsigned)cluster, stream, maps[0], maps[1], maps[2], a);
 }
 
 }  // namespace
@@ -969,10 +964,10 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     const void* x = order ? in.workspace : in.x;
     const int64_t x_rows = order ? in.rows : in.x_rows, x_row = order || x_rows == 1 ? ordered_stride : in.x_stride;
     if (order) {
-        const dim3 grid((unsigned)std::min<int64_t>(in.rows, 16 * (int64_t)sms), 1);
-        order_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(in.x), in.x_stride, in.row_index, in.offsets, (int)in.groups, (int)in.rows,
-                                                    (int)in.x_rows, (int)in.K, static_cast<uint16_t*>(in.workspace), ordered_stride, in.status);
-        SFB_CUDA_CHECK(cudaGetLastError());
+        const int rc = launch_after(order_rows_kernel, (unsigned)std::min<int64_t>(in.rows, 8 * (int64_t)sms), 256, 0, 1, stream,
+                                    static_cast<const uint16_t*>(in.x), in.x_stride, in.row_index, in.offsets, (int)in.groups, (int)in.rows,
+                                    (int)in.x_rows, (int)in.K, static_cast<uint16_t*>(in.workspace), ordered_stride, in.status);
+        if (rc != SFB_OK) return rc;
     }
     // rows of out and residual in pieces of `cols` values where all of them start on one
     const int cols = a.gated ? 2 : 4, piece = cols * (a.out_f32 ? 4 : 2);

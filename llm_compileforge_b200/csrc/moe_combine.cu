@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(288) moe_combine_kernel(const CombineArgs a, i
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty + 8 * threadIdx.x), "r"(summing));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    let_next_start();
+    wait_for_previous();
     __syncthreads();
     // this block's segment of the rows, its tokens and, one ahead, their rows
     const unsigned first = blockIdx.x / segments, s = blockIdx.x - first * segments, step = gridDim.x / segments, tokens = (unsigned)a.tokens;
@@ -209,9 +211,7 @@ int launch(const CombineArgs& a, cudaStream_t stream) {
     const int threads = 32 * (1 + segment / 512), smem = kSlots * segment;
     const int64_t resident = (int64_t)sms * std::min(2048 / threads, 229376 / (smem + 2048));
     const int64_t blocks = segments * std::max<int64_t>(1, std::min(a.tokens, resident / segments));
-    moe_combine_kernel<T><<<(unsigned)blocks, threads, smem, stream>>>(a, segment, (unsigned)segments);
-    SFB_CUDA_CHECK(cudaGetLastError());
-    return SFB_OK;
+    return launch_after(moe_combine_kernel<T>, (unsigned)blocks, (unsigned)threads, smem, 1, stream, a, segment, (unsigned)segments);
 }
 
 }  // namespace

@@ -77,10 +77,6 @@ __device__ void place_rows(const RouteArgs& a, const uint32_t (*mask)[kWords], c
     for (int64_t r = total + (int64_t)blockIdx.x * kRouteThreads + threadIdx.x; r < all; r += (int64_t)gridDim.x * kRouteThreads) a.token_rows[r] = -1;
 }
 
-// The dependent launch may start; what it reads it waits for.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // A lane's logits lane, lane + 32, ... with their rounds of selection.
 template <typename T, int PER>
 struct Lane {
@@ -167,6 +163,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_select_kernel(const Route
     const int n_tokens = (int)min((int64_t)kRouteTokens, a.tokens - t0);
     let_next_start();
     for (int i = threadIdx.x; i < 32 * PER * kWords; i += kRouteThreads) (&mask[0][0])[i] = 0u;
+    wait_for_previous();
     __syncthreads();
 
     for (int t = warp; t < n_tokens; t += kWarps) {
@@ -244,6 +241,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
     const int n_tokens = (int)min((int64_t)kRouteTokens, a.tokens - t0), blocks = (int)gridDim.x;
     for (int i = threadIdx.x; i < a.experts * kWords; i += kRouteThreads) (&mask[0][0])[i] = 0u;
     for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] = before[e] = 0;
+    let_next_start();
     __syncthreads();
     wait_for_previous();
     for (int i = threadIdx.x; i < n_tokens * a.top_k; i += kRouteThreads) {
@@ -283,37 +281,27 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
 }
 
 template <typename T>
-void launch_select(const RouteArgs& a, unsigned blocks, cudaStream_t stream) {
-    if (a.experts <= 64) route_select_kernel<T, 2><<<blocks, kRouteThreads, 0, stream>>>(a);
-    else if (a.experts <= 128) route_select_kernel<T, 4><<<blocks, kRouteThreads, 0, stream>>>(a);
-    else if (a.experts <= 256) route_select_kernel<T, 8><<<blocks, kRouteThreads, 0, stream>>>(a);
-    else route_select_kernel<T, 32><<<blocks, kRouteThreads, 0, stream>>>(a);
+int launch_select(const RouteArgs& a, unsigned blocks, cudaStream_t stream) {
+    auto go = [&](auto kernel) { return launch_after(kernel, blocks, kRouteThreads, 0, 1, stream, a); };
+    if (a.experts <= 64) return go(route_select_kernel<T, 2>);
+    if (a.experts <= 128) return go(route_select_kernel<T, 4>);
+    if (a.experts <= 256) return go(route_select_kernel<T, 8>);
+    return go(route_select_kernel<T, 32>);
 }
 
 }  // namespace
 
 int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
     const unsigned blocks = (unsigned)ceil_div(a.tokens, (int64_t)kRouteTokens);
-    if (a.dtype == SFB_F32) launch_select<float>(a, blocks, stream);
-    else if (a.dtype == SFB_BF16) launch_select<__nv_bfloat16>(a, blocks, stream);
-    else launch_select<__half>(a, blocks, stream);
-    SFB_CUDA_CHECK(cudaGetLastError());
-    if (blocks == 1) return SFB_OK;
+    const int rc = a.dtype == SFB_F32 ? launch_select<float>(a, blocks, stream)
+                   : a.dtype == SFB_BF16 ? launch_select<__nv_bfloat16>(a, blocks, stream) : launch_select<__half>(a, blocks, stream);
+    if (rc != SFB_OK || blocks == 1) return rc;
     const bool scanned = blocks > kSumBlocks;
     if (scanned) {
         route_scan_kernel<<<(unsigned)ceil_div((int64_t)a.experts, (int64_t)32), 1024, 0, stream>>>(a.counts, (int)blocks, a.experts);
         SFB_CUDA_CHECK(cudaGetLastError());
     }
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its blocks start while the selecting ones end
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kRouteThreads);
-    cfg.stream = stream;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    SFB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, route_place_kernel, a, scanned));
-    return SFB_OK;
+    return launch_after(route_place_kernel, blocks, kRouteThreads, 0, 1, stream, a, scanned);
 }
 
 }  // namespace sfb
