@@ -4,7 +4,7 @@
 // (larger logit, lower index); their weights are exp(l - max) over the sum of the chosen ones (renormalize) or of all
 // experts.  The sort is stable (expert, then token): row of (t, e) = offsets[e] + number of tokens before t that chose e.
 //
-// One warp selects for one token: a lane holds every 32nd logit as a key whose unsigned order is the float order, sorted;
+// One warp selects for one token: a lane holds consecutive logits as keys whose unsigned order is the float order, sorted;
 // top_k rounds of a warp-wide maximum over the lanes' first keys take the winners.  16-bit logits carry their index in the
 // key's lower half (complemented: the lower index wins), so a round is one reduction; fp32 needs a second for the index.
 // A token chooses an expert at most once, so what a block of 128 tokens chose is one 128-bit mask per expert: a token's rank
@@ -15,6 +15,7 @@
 // Bound: launch latency for few tokens, the selection rounds' instructions for many.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "linear.cuh"
 
@@ -77,33 +78,41 @@ __device__ void place_rows(const RouteArgs& a, const uint32_t (*mask)[kWords], c
     for (int64_t r = total + (int64_t)blockIdx.x * kRouteThreads + threadIdx.x; r < all; r += (int64_t)gridDim.x * kRouteThreads) a.token_rows[r] = -1;
 }
 
-// A lane's logits lane, lane + 32, ... with their rounds of selection.
+// A lane's PER consecutive logits with their rounds of selection.
 template <typename T, int PER>
 struct Lane {
     static constexpr bool kPacked = sizeof(T) == 2;  // key << 16 | ~index; a 16-bit float's key has 16 bits
     uint32_t key[PER];
     int index[kPacked ? 1 : PER];
 
-    __device__ __forceinline__ void load(const T* l, int lane, int experts) {
+    __device__ __forceinline__ void load(const T* l, int lane, int experts, bool vector) {
+        T v[PER];
+        if (vector && (lane + 1) * PER <= experts) {
+            using Vec = std::conditional_t<sizeof(T) * PER == 4, uint32_t, std::conditional_t<sizeof(T) * PER == 8, uint2, uint4>>;
+            constexpr int kVecs = sizeof(T) * PER <= 16 ? 1 : (int)(sizeof(T) * PER / 16);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) reinterpret_cast<Vec*>(v)[i] = reinterpret_cast<const Vec*>(l + lane * PER)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = lane * PER + i < experts ? l[lane * PER + i] : from_float<T>(-INFINITY);
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = lane + 32 * i;
-            const float v = e < experts ? to_float(l[e]) : -INFINITY;
-            uint32_t k = order_key(v);
+            const int e = lane * PER + i;
             if constexpr (kPacked) {
-                if (k) k = pack(v, e);
+                key[i] = half_key(*reinterpret_cast<const uint16_t*>(&v[i]), e);
             } else {
+                key[i] = order_key(to_float(v[i]));
                 index[i] = e;
             }
-            key[i] = k;
         }
     }
-    // The 16-bit key of a 16-bit float, never 0 for a candidate (only -inf and NaNs lie below the lowest)
-    static __device__ __forceinline__ uint32_t pack(float v, int e) {
-        const T t = from_float<T>(v + 0.f);
-        uint32_t b = *reinterpret_cast<const uint16_t*>(&t);
-        b = b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
-        return b << 16 | (0xffffu - (uint32_t)e);
+    // The ordered bits of a 16-bit float, -0 as +0, over the complement of the index; 0 for -inf and NaNs.
+    static __device__ __forceinline__ uint32_t half_key(uint32_t b, int e) {
+        constexpr uint32_t kInf = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+        if (b == 0x8000u) b = 0u;
+        const uint32_t k = b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
+        return (b & 0x7fffu) > kInf || b == (0x8000u | kInf) ? 0u : k << 16 | (0xffffu - (uint32_t)e);
     }
     static __device__ __forceinline__ float value(uint32_t k) {
         if constexpr (kPacked) {
@@ -166,37 +175,64 @@ __global__ void __launch_bounds__(kRouteThreads) route_select_kernel(const Route
     wait_for_previous();
     __syncthreads();
 
-    for (int t = warp; t < n_tokens; t += kWarps) {
-        Lane<T, PER> l;
-        l.load(static_cast<const T*>(a.logits) + (t0 + t) * a.logits_stride, lane, a.experts);
-        l.sort();
-        const uint32_t top = __reduce_max_sync(0xffffffffu, l.key[0]);
-        const float top_value = Lane<T, PER>::value(top);
-        float sum = 0.f;
-        if (!a.renormalize && top) {
+    // rows that start on a lane's piece are read piece by piece
+    constexpr uint32_t kPiece = sizeof(T) * PER < 16 ? sizeof(T) * PER : 16;
+    const bool vector = reinterpret_cast<uintptr_t>(a.logits) % kPiece == 0 && a.logits_stride * sizeof(T) % kPiece == 0;
+    // N tokens at a time: their rounds run beside one another
+    auto select = [&](int t, auto count) {
+        constexpr int N = decltype(count)::value;
+        Lane<T, PER> l[N];
+        float top_value[N], sum[N];
+        int my_id[N];
+        uint32_t my_key[N];
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (l.key[i]) sum += exp_below(Lane<T, PER>::value(l.key[i]), top_value);
-            sum = warp_sum(sum);
+        for (int i = 0; i < N; ++i) {
+            const int u = min(t + i * kWarps, n_tokens - 1);  // (past the end: the last token again, not written)
+            l[i].load(static_cast<const T*>(a.logits) + (t0 + u) * a.logits_stride, lane, a.experts, vector);
+            l[i].sort();
+            my_id[i] = -1;
+            my_key[i] = 0;
+            sum[i] = 0.f;
         }
-        int my_id = -1;
-        uint32_t my_key = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, l[i].key[0]);
+            top_value[i] = Lane<T, PER>::value(top);
+            if (!a.renormalize && top) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (l[i].key[k]) sum[i] += exp_below(Lane<T, PER>::value(l[i].key[k]), top_value[i]);
+                sum[i] = warp_sum(sum[i]);
+            }
+        }
+#pragma unroll 1
         for (int j = 0; j < a.top_k; ++j) {
-            int e;
-            const uint32_t m = l.take(e);
-            if (!m) break;
-            if (lane == j) { my_id = e; my_key = m; }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int e;
+                const uint32_t m = l[i].take(e);
+                if (lane == j) { my_id[i] = e; my_key[i] = m; }
+            }
         }
-        const float my_weight = my_id >= 0 ? exp_below(Lane<T, PER>::value(my_key), top_value) : 0.f;
-        if (a.renormalize) sum = warp_sum(my_weight);
-        if (lane < a.top_k) {
-            const int64_t o = (t0 + t) * a.top_k + lane;
-            a.ids[o] = my_id;
-            a.weights[o] = my_id >= 0 ? my_weight / sum : 0.f;
-            ids[t * a.top_k + lane] = (int16_t)my_id;
-            if (my_id >= 0) atomicOr(&mask[my_id][t >> 5], 1u << (t & 31));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = t + i * kWarps;
+            if (!my_key[i]) my_id[i] = -1;
+            const float w = my_id[i] >= 0 ? exp_below(Lane<T, PER>::value(my_key[i]), top_value[i]) : 0.f;
+            if (a.renormalize) sum[i] = warp_sum(w);
+            if (lane < a.top_k && u < n_tokens) {
+                const int64_t o = (t0 + u) * a.top_k + lane;
+                a.ids[o] = my_id[i];
+                a.weights[o] = my_id[i] >= 0 ? w / sum[i] : 0.f;
+                ids[u * a.top_k + lane] = (int16_t)my_id[i];
+                if (my_id[i] >= 0) atomicOr(&mask[my_id[i]][u >> 5], 1u << (u & 31));
+            }
         }
-    }
+    };
+    if (PER > 8 || n_tokens <= kWarps)
+        for (int t = warp; t < n_tokens; t += kWarps) select(t, std::integral_constant<int, 1>{});
+    else
+        for (int t = warp; t < n_tokens; t += 2 * kWarps) select(t, std::integral_constant<int, PER <= 8 ? 2 : 1>{});
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
         const int c = mask_count(mask[e]);
@@ -243,11 +279,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
     for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] = before[e] = 0;
     let_next_start();
     __syncthreads();
-    wait_for_previous();
-    for (int i = threadIdx.x; i < n_tokens * a.top_k; i += kRouteThreads) {
-        const int e = a.ids[t0 * a.top_k + i], t = i / a.top_k;
-        ids[i] = (int16_t)e;
-        if (e >= 0) atomicOr(&mask[e][t >> 5], 1u << (t & 31));
+    // this block's assignments on their way while the counts are added
+    constexpr int kEach = kRouteTokens * kMaxTopK / kRouteThreads;
+    int mine[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = threadIdx.x + j * kRouteThreads;
+        mine[j] = i < n_tokens * a.top_k ? a.ids[t0 * a.top_k + i] : -1;
     }
     if (scanned) {
         for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
@@ -268,6 +306,14 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
             atomicAdd(&start[e], all);
             atomicAdd(&before[e], below);
         }
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = threadIdx.x + j * kRouteThreads;
+        if (i >= n_tokens * a.top_k) break;
+        const int t = i / a.top_k;
+        ids[i] = (int16_t)mine[j];
+        if (mine[j] >= 0) atomicOr(&mask[mine[j]][t >> 5], 1u << (t & 31));
     }
     __syncthreads();
     block_exclusive_sum(start, a.experts);
@@ -301,7 +347,11 @@ int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
         route_scan_kernel<<<(unsigned)ceil_div((int64_t)a.experts, (int64_t)32), 1024, 0, stream>>>(a.counts, (int)blocks, a.experts);
         SFB_CUDA_CHECK(cudaGetLastError());
     }
-    return launch_after(route_place_kernel, blocks, kRouteThreads, 0, 1, stream, a, scanned);
+    // launched in the plain way: blocks that start while the selecting ones run crowd onto the SMs those leave free (22 us
+    // against 14 for 16384 tokens of 128 experts)
+    route_place_kernel<<<blocks, kRouteThreads, 0, stream>>>(a, scanned);
+    SFB_CUDA_CHECK(cudaGetLastError());
+    return SFB_OK;
 }
 
 }  // namespace sfb
