@@ -95,3 +95,42 @@ def test_route_workspace_query():
     assert ops.moe_route_workspace_bytes(128 * 3, 64) >= 3 * 64 * 4
     with pytest.raises(ValueError):
         ops.moe_route_workspace_bytes(-1, 4)
+
+
+def test_plan_of_tile_shapes():
+    plan = ops.linear_plan
+    # one token against 32 column tiles: their K is shared so that the SMs are full, in one round
+    p = plan(1, 4096, 4096)
+    assert p["tokens"] == 32 and not p["pair"] and 96 <= p["split"] * p["feature_tiles"] <= 148
+    # many tokens: clusters of two; nothing to order
+    assert plan(8192, 8192, 8192) == dict(tokens=256, pair=1, split=1, order=0, blocks_an_sm=1, feature_tiles=32)
+    assert plan(8192, 8192, 8192, gated=True)["feature_tiles"] == 64
+    # a decode batch whose tiles outnumber the SMs: two blocks an SM
+    p = plan(64, 4096, 14336, gated=True)
+    assert p["blocks_an_sm"] == 2 and p["tokens"] == 64 and p["split"] == 1
+    # rows by index: ordered first where groups have many, but only with room for it
+    assert plan(16384, 4096, 1792, groups=32, gated=True, indexed=True)["order"] == 1
+    p = plan(16384, 4096, 1792, groups=32, gated=True, indexed=True, has_workspace=False)
+    assert p["order"] == 0 and p["pair"] == 0
+    assert plan(128, 2048, 1408, groups=32, gated=True, indexed=True)["order"] == 0
+    # no split finer than K has steps, every shape one that exists
+    for rows in (1, 7, 33, 100, 129, 500, 3000):
+        for k in (8, 64, 72, 1000, 8192):
+            for n in (8, 128, 1000, 14336):
+                for groups in (0, 1, 16, 300):
+                    p = plan(rows, k, n, groups=groups, indexed=groups > 1)
+                    assert p["tokens"] in (32, 64, 128, 256) and p["pair"] == (p["tokens"] == 256) and 1 <= p["split"] <= min(8, -(-k // 64))
+                    assert p == plan(rows, k, n, groups=groups, indexed=groups > 1)  # the kept one is the priced one
+    for bad in ((0, 8, 8), (8, 0, 8), (8, 8, 0)):
+        with pytest.raises(ValueError):
+            plan(*bad)
+    with pytest.raises(ValueError):
+        plan(8, 8, 8, groups=2000)
+
+
+def test_ordering_workspace_query():
+    assert ops.grouped_linear_workspace_bytes(100, 64, 32) == 0  # few rows a group: gathered
+    assert ops.grouped_linear_workspace_bytes(4096, 65, 32) == 4096 * 72 * 2
+    assert ops.grouped_linear_workspace_bytes(4096, 65, 32, indexed=False) == 0
+    with pytest.raises(ValueError):
+        ops.grouped_linear_workspace_bytes(4096, 65, 0)

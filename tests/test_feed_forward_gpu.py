@@ -183,6 +183,42 @@ def test_linear_keeps_infinities_and_nan_in_their_rows():
         assert torch.equal(got[keep], ops.fused_linear(x[keep], w)) if rows == 5 else torch.isfinite(got[keep]).all()
 
 
+@pytest.mark.parametrize("rows", [5, 40, 100, 200, 600, 1100])
+@pytest.mark.parametrize("k,n", [(4096, 256), (2048, 101)])
+def test_linear_every_output_form(rows, k, n):
+    """fp32 and 16-bit results in whole pieces and value by value, on the shapes that split K, walk tiles and pair blocks."""
+    pad = (-n) % 8 if n % 8 else 0
+    k += (-(k + pad)) % 8
+    for gated in (False, True):
+        check_linear(rows, k, n, gated=gated, act="silu", bias=True, residual=True, out_dtype=F32, pad=pad)
+        check_linear(rows, k, n, gated=gated, act="relu", residual=True, dtype=F16, pad=pad)
+
+
+def test_linear_broadcast_and_unaligned_operands():
+    from llm_compileforge_b200 import ops
+
+    g = gen(21)
+    w, b = make(g, 136, 96, std=0.1), make(g, 96)
+    for rows in (6, 300):
+        x = make(g, rows, 144)
+        one = x[:1, :136].expand(rows, 136)  # rows that all lie in one place
+        want, tol = linear64(one, w, b)
+        assert_rounded(ops.fused_linear(one, w, b), want, tol)
+        r = make(g, 1, 96).expand(rows, 96)
+        want, tol = linear64(x[:, :136], w, r=r)
+        assert_rounded(ops.fused_linear(x[:, :136], w, residual=r), want, tol)
+        for shift in (1, 3):  # bases off 16 bytes
+            xs = x[:, shift:136 + shift]
+            want, tol = linear64(xs, w, b)
+            assert_rounded(ops.fused_linear(xs, w, b), want, tol)
+        flat = torch.zeros(rows * 100 + 8, dtype=BF16, device="cuda")
+        out = flat[1:1 + rows * 100].view(rows, 100)[:, 3:99]  # rows of out off every piece
+        ops.fused_linear(x[:, :136], w, b, out=out)
+        want, tol = linear64(x[:, :136], w, b)
+        assert_rounded(out, want, tol)
+        assert flat[0] == 0 and (flat[1 + rows * 100:] == 0).all()
+
+
 # ── grouped ──────────────────────────────────────────────────────────────────
 def offsets_of(counts, first=0):
     at = [first]
@@ -294,6 +330,51 @@ def test_grouped_bad_offsets_and_indices_are_flagged_and_stay_inside():
         keep = [i for i in range(40) if i not in (7, 33)]
         fine = ops.grouped_linear(x, w, offsets_of([10, 10, 10, 10]), row_index=torch.arange(40, dtype=torch.int32, device="cuda"))
         assert torch.equal(got[keep], fine[keep])
+
+
+def test_grouped_many_groups_of_many_rows():
+    for counts in ([90 + i % 40 for i in range(1024)], [300] * 200 + [0] * 57):
+        check_grouped(counts, 64, 72, gather=True, x_rows=5000)
+        check_grouped(counts, 64, 40, gated=True, act="silu", layout="nk")
+
+
+def test_grouped_without_room_to_order_rows():
+    from llm_compileforge_b200 import ops
+
+    g = gen(31)
+    counts = [140, 0, 260, 33]
+    x, w, v = make(g, 200, 328), make(g, 4, 328, 264, std=0.06), make(g, 4, 328, 264, std=0.06)
+    index = torch.randint(0, 200, (sum(counts),), generator=g, device="cuda", dtype=torch.int32)
+    for gate in (None, v):
+        ordered = ops.grouped_linear(x, w, offsets_of(counts), row_index=index, up_weight=gate)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        small = torch.empty(16, dtype=torch.uint8, device="cuda")
+        assert ops.grouped_linear_workspace_bytes(sum(counts), 328, 4) > 16
+        gathered = ops.grouped_linear(x, w, offsets_of(counts), row_index=index, up_weight=gate, workspace=small, status=status)
+        at = 0
+        for i, m in enumerate(counts):
+            want, tol = linear64(x[index[at:at + m].long()], w[i], None, "none", None if gate is None else gate[i])
+            assert_rounded(gathered[at:at + m], want, tol)
+            assert_rounded(ordered[at:at + m], want, tol)
+            at += m
+        assert status.item() == 0
+
+
+def test_grouped_broadcast_over_the_experts_and_nan_rows():
+    from llm_compileforge_b200 import ops
+
+    g = gen(32)
+    for counts in ([7, 0, 20, 3], [200, 90, 0, 130]):
+        x = make(g, sum(counts), 64)
+        w, b = make(g, 1, 64, 72, std=0.1).expand(4, 64, 72), make(g, 1, 72).expand(4, 72)
+        want, tol = linear64(x, w[0], b[0])
+        assert_rounded(ops.grouped_linear(x, w, offsets_of(counts), b), want, tol)
+        w = make(g, 4, 64, 72, std=0.1)
+        clean = ops.grouped_linear(x, w, offsets_of(counts), b)
+        x[counts[0] - 1] = math.nan  # the last row of a group: its tile also covers the next group's first rows
+        got = ops.grouped_linear(x, w, offsets_of(counts), b)
+        keep = [i for i in range(sum(counts)) if i != counts[0] - 1]
+        assert got[counts[0] - 1].isnan().all() and torch.equal(got[keep], clean[keep])
 
 
 # ── routing ──────────────────────────────────────────────────────────────────
@@ -505,3 +586,39 @@ def test_captured_graphs_streams_and_changed_inputs():
             other = moe_block(be, x, router, w1, w3, w2, top_k)[-1]
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(other, want)
+
+
+def test_calls_on_two_streams_at_once():
+    import llm_compileforge_b200 as pkg
+
+    be, g, top_k = pkg.B200Backend(), gen(14), 2
+    router, w1, w3, w2 = make(g, 128, 8, std=0.2), make(g, 8, 128, 200, std=0.1), make(g, 8, 128, 200, std=0.1), make(g, 8, 200, 128, std=0.1)
+    xs = [make(g, 400, 128) for _ in range(2)]
+    want = [moe_block(be, x, router, w1, w3, w2, top_k)[-1] for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(moe_block(be, xs[i], router, w1, w3, w2, top_k)[-1])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_results_behind_other_kernels():
+    """A chain of calls with torch kernels that write their inputs right before them, without a pause: each call waits for what it reads."""
+    from llm_compileforge_b200 import ops
+
+    g = gen(15)
+    x, w = make(g, 64, 512), make(g, 512, 512, std=0.04)
+    want = x
+    for _ in range(6):
+        want = ops.fused_linear((want * 0.5).contiguous(), w, residual=want)
+        torch.cuda.synchronize()
+    for _ in range(10):
+        h = x
+        for _ in range(6):
+            h = ops.fused_linear((h * 0.5).contiguous(), w, residual=h)
+        assert torch.equal(h, want)
