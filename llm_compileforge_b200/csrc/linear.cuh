@@ -92,6 +92,16 @@ int launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int smem, 
     return SFB_OK;
 }
 
+// After a wait that ran out: copies may still be on their way into this block's shared memory, so the thread stays a while (20 ms,
+// thousands of times what a copy takes) before the block may end.
+__device__ __forceinline__ void settle() {
+    uint64_t begun, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(begun));
+    do {
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    } while (now - begun < 20000000);
+}
+
 // Group offsets come from the device and are not trusted: each is clamped to [0, rows], and one below an offset before it
 // counts as that one.  Groups then never overlap or leave the rows, whatever the array holds.
 __device__ __forceinline__ int group_offset(int raw, int before, int rows) { return max(before, min(raw, rows)); }

@@ -467,7 +467,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 quad = make_int4(r[0], r[1], r[2], r[3]);
             }
             for (int k = k_first; k < k_end; k += sub) {
-                if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
+                // (all lanes step together: one without a box that fell behind would miss a phase that it waits for)
+                if (!__all_sync(0xffffffffu, mbar_wait(bar(B_EMPTY + s), ephase))) { timed_out = true; break; }
                 const int end = min(k + (int)sub, k_end);
                 if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), (end - k) * bytes);
                 uint32_t dst = place + s * stage_bytes;
@@ -478,7 +479,6 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 if (++s == stages) { s = 0; ephase ^= 1; }
             }
         }
-        timed_out = __any_sync(0xffffffffu, timed_out);
     } else if (warp == kMmaWarp) {
         // ============================ MMA issuer ==============================
         if (lane == 0 && (!PAIR || rank == 0)) {
@@ -762,6 +762,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         }
         timed_out = !ok;
     }
+    if (timed_out) settle();
     if (timed_out && a.status && lane == 0) atomicOr(a.status, SFB_STATUS_WAIT_TIMEOUT);
     // ---- teardown: every warp arrives here; in a cluster no block leaves while another may still use its shared memory
     __syncwarp();

@@ -4,7 +4,7 @@
 // order of j, one rounding; no atomics, so the same inputs give the same bits.
 // Bound by HBM: tokens * top_k rows of y in, a row of out (and of residual) per token.  Rows lie anywhere, so the bandwidth
 // hangs on how many of them are in flight: one warp of a thread block issues bulk copies of whole row segments (up to 4 KB)
-// into a ring of 24 slots in shared memory, lane j the j-th row of the token, and runs ahead of the warps that sum them by
+// into a ring of 18 slots in shared memory, lane j the j-th row of the token, and runs ahead of the warps that sum them by
 // as many tokens as the ring holds.  (With 16-byte loads into registers instead, eight rows a lane, the compiler either
 // serialised them or left too few warps an SM: 2.3 to 4.5 TB/s at 8192 tokens of 8 rows of 4096.)
 // Rows that bulk copies cannot address (not on 16 bytes) go value by value through registers.
@@ -17,7 +17,7 @@
 namespace sfb {
 namespace {
 
-constexpr int kSlots = 24, kBatch = 16;  // rows in flight; rows issued together (fewer than the slots: see below)
+constexpr int kSlots = 18, kBatch = 16;  // rows in flight; rows issued together
 constexpr int kSegmentBytes = 4096;      // of a row, at most: eight warps of 32 lanes of 16 bytes
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -125,8 +125,8 @@ __global__ void __launch_bounds__(288) moe_combine_kernel(const CombineArgs a, i
         const uint32_t mask = __ballot_sync(0xffffffffu, inside(a, rows.row));
         if (warp == 0) {
             if (s == 0 && a.status && rows.row != -1 && !inside(a, rows.row)) atomicOr(a.status, SFB_STATUS_BAD_ROW_INDEX);
-            // A lane that waits for its slot holds the others up, so what it waits for must not hang on their copies: the
-            // slots that a batch takes were all filled before it
+            // A batch is no larger than the ring, and no lane begins the next one before every lane is through with this one: each
+            // slot that a lane waits for has then been filled before, and the parity it asks for cannot be the one before last
             for (int j0 = 0; j0 < a.top_k; j0 += kBatch) {
                 const uint32_t batch = mask >> j0 & ((1u << kBatch) - 1u);
                 const int rank = __popc(batch & ((1u << (lane & (kBatch - 1))) - 1u));
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(288) moe_combine_kernel(const CombineArgs a, i
                     ok = mbar_wait(empty + 8 * mine, p ^ 1);
                     if (ok) bulk_load(ring0 + mine * segment_bytes, y + rows.row * y_bytes, bytes, full + 8 * mine);
                 }
+                __syncwarp();
                 skip(__popc(batch));
             }
             if (residual) {
@@ -165,6 +166,7 @@ __global__ void __launch_bounds__(288) moe_combine_kernel(const CombineArgs a, i
         ok = __all_sync(0xffffffffu, ok);
         if (ok && mine < bytes) *reinterpret_cast<uint4*>(out + token * out_bytes + mine) = rounded<T>(sum);
     }
+    if (!ok) settle();
     if (!ok && a.status && lane == 0) atomicOr(a.status, SFB_STATUS_WAIT_TIMEOUT);
 }
 

@@ -483,6 +483,25 @@ def test_combine(dtype, tokens, top_k, h):
     assert (view[:, :8] == 2).all() and (view[:, 8 + h:] == 2).all()
 
 
+@pytest.mark.parametrize("tokens,top_k,h,with_residual", [(2000, 32, 1024, False), (3000, 32, 256, True), (1500, 20, 2048, True), (1200, 17, 512, False), (5000, 16, 128, True)])
+def test_combine_many_tokens_of_many_rows(tokens, top_k, h, with_residual):
+    """Every token's rows go round the ring more than once, in several batches, many tokens after one another in a block."""
+    from llm_compileforge_b200 import ops
+
+    g = gen(tokens + h)
+    y, weights = make(g, tokens * top_k, h), torch.rand((tokens, top_k), generator=g, device="cuda")
+    positions = torch.randperm(tokens * top_k, generator=g, device="cuda").to(torch.int32).view(tokens, top_k)
+    r = make(g, tokens, h) if with_residual else None
+    terms = weights.double()[..., None] * y[positions.long()].double()
+    want, size = terms.sum(1), terms.abs().sum(1)
+    if with_residual:
+        want, size = want + r.double(), size + r.double().abs()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        assert_rounded(ops.moe_combine(y, positions, weights, residual=r, status=status), want, (top_k + 1) * 2.0 ** -24 * size)
+    assert status.item() == 0
+
+
 def test_combine_bad_positions_empty_rows_and_no_tokens():
     from llm_compileforge_b200 import _lib, ops
 
