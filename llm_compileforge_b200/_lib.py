@@ -139,7 +139,33 @@ def load() -> ctypes.CDLL:
     lib.sfb_peer_signal_wait.restype = c_int
     lib.sfb_peer_signal_wait.argtypes = [POINTER(c_void_p), c_int, c_int, ctypes.c_uint32, c_int, c_void_p, c_void_p]
     _lib = lib
+    _bind_calls(lib)
     return lib
+
+
+class _NoCalls:
+    """Stands in for the ``_calls`` module where it is not built: no call is one of its."""
+
+    @staticmethod
+    def linear(*args):
+        return None
+
+    grouped = route = combine = linear
+
+
+calls = None  # the quick way into the library (csrc/calls.cpp), set when the library is loaded
+
+
+def _bind_calls(lib: ctypes.CDLL) -> None:
+    global calls
+    try:
+        from . import _calls
+    except ModuleNotFoundError:
+        calls = _NoCalls
+        return
+    names = ("sfb_fused_linear", "sfb_grouped_linear", "sfb_grouped_linear_workspace_bytes", "sfb_moe_route", "sfb_moe_route_workspace_bytes", "sfb_moe_combine")
+    _calls.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in names))
+    calls = _calls
 
 
 def _optional(lib: ctypes.CDLL) -> None:

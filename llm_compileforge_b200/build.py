@@ -5,6 +5,8 @@
 nvcc cross-compiles without a GPU.  Each ``csrc/*.cu`` becomes an object under
 ``csrc/_obj`` (rebuilt only when it or a header changed) and the objects are
 linked, with the static CUDA runtime, into ``llm_compileforge_b200/libsfb.so``.
+``csrc/calls.cpp`` becomes the extension module ``_calls`` beside it (host code
+against PyTorch's headers: the quick way from Python into the library).
 """
 
 from __future__ import annotations
@@ -12,6 +14,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -68,7 +71,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose or res.returncode:
             sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
         if res.returncode:
-            raise RuntimeError(f"nvcc failed for {cmd[-3]}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed for {cmd[-3]}")
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as pool:
         list(pool.map(run, jobs))
@@ -76,7 +79,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if jobs or force or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         cmd = [nvcc, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static"]
         run(cmd)
+    if not os.environ.get("SFB_LIB_OUT"):
+        build_calls(force, run)
     return LIB
+
+
+def calls_path() -> str:
+    return os.path.join(PKG, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_calls(force: bool, run) -> None:
+    src, out = os.path.join(CSRC, "calls.cpp"), calls_path()
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), _headers_mtime()):
+        return
+    import torch
+    from torch.utils import cpp_extension
+
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         *(f"-I{d}" for d in include), src, "-o", out, *(f"-L{d}" for d in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
 
 
 if __name__ == "__main__":

@@ -488,6 +488,20 @@ def _rows(what: str, t: torch.Tensor, n: int) -> torch.Tensor:
         raise ValueError(f"{what}: strides {t.stride()} do not make rows of {n}") from None
 
 
+def _quick(name: str):
+    """A function of the quick way into the library: the call's result, or None where the checks and words below are needed."""
+    if _lib.calls is None:
+        _lib.load()
+    return getattr(_lib.calls, name)
+
+
+def _done(got):
+    """What a quick call answered with: the result, or a status to raise."""
+    if type(got) is int:
+        check(got)
+    return got
+
+
 def _activation(what: str, name: str) -> int:
     try:
         return ACTIVATIONS[name]
@@ -504,6 +518,10 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     :data:`ACTIVATIONS`.  The result has ``x``'s type, or float32 with ``out_dtype=torch.float32``; ``out`` may be the residual
     itself.  fp32 accumulation, one rounding.  bf16 / fp16 operands whose rows are 16-byte aligned run on the tensor
     cores, all others on the CUDA cores.  ``status`` (int32, device) collects status bits."""
+    if type(activation) is str and (out_dtype is None or out_dtype is torch.float32):
+        got = _quick("linear")(x, weight, bias, up_weight, up_bias, residual, out, status, ACTIVATIONS.get(activation, -1), out_dtype is not None)
+        if got is not None:
+            return _done(got)
     xs, ws, dtype = x.shape, weight.shape, x.dtype
     if len(ws) != 2 or not xs or xs[-1] != ws[0]:
         raise ValueError(f"fused_linear: x [..., K] and weight [K, N], got {tuple(xs)} and {tuple(ws)}")
@@ -569,6 +587,11 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     they were (in a fresh result: undefined).  ``workspace`` (uint8, :func:`grouped_linear_workspace_bytes`; allocated when
     missing) holds the rows of ``x`` in the order of ``row_index`` where groups have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
     indices outside their range."""
+    if type(activation) is str and (out_dtype is None or out_dtype is torch.float32):
+        got = _quick("grouped")(x, weight, group_offsets, bias, up_weight, up_bias, row_index, out, workspace, status, ACTIVATIONS.get(activation, -1),
+                                out_dtype is not None)
+        if got is not None:
+            return _done(got)
     xs, ws, dtype = x.shape, weight.shape, x.dtype
     if len(xs) != 2 or len(ws) != 3 or xs[1] != ws[1]:
         raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(xs)} and {tuple(ws)}")
@@ -631,6 +654,9 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, wor
     over the chosen experts (``renormalize``) or over all, and the assignments sorted by expert, then token.  A logit of
     ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8,
     :func:`moe_route_workspace_bytes`) is allocated when missing."""
+    got = _quick("route")(logits, top_k, renormalize, workspace)
+    if got is not None:
+        return MoeRouting._make(_done(got))
     ls = logits.shape
     if len(ls) != 2:
         raise ValueError(f"moe_route: logits [T, E], got {tuple(ls)}")
@@ -664,6 +690,9 @@ def moe_combine(y: torch.Tensor, positions: torch.Tensor, weights: torch.Tensor,
     """``out[t] = sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])``: every token's experts' rows (``y [R, H]``, the last
     :func:`grouped_linear`'s result) back to the token; ``positions`` int32 and ``weights`` float32 ``[T, top_k]`` are
     :func:`moe_route`'s.  A position of -1 adds nothing.  fp32 sums in the order of j, one rounding; ``out`` may be the residual."""
+    got = _quick("combine")(y, positions, weights, residual, out, status)
+    if got is not None:
+        return _done(got)
     ys, ps, dtype = y.shape, positions.shape, y.dtype
     if len(ys) != 2 or len(ps) != 2 or ps != weights.shape:
         raise ValueError(f"moe_combine: y [R, H], positions and weights [T, k], got {tuple(ys)}, {tuple(ps)}, {tuple(weights.shape)}")

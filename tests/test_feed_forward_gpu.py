@@ -641,3 +641,71 @@ def test_results_behind_other_kernels():
         for _ in range(6):
             h = ops.fused_linear((h * 0.5).contiguous(), w, residual=h)
         assert torch.equal(h, want)
+
+
+# ── the two ways from Python into the library ────────────────────────────────
+def test_both_ways_into_the_library_agree(monkeypatch):
+    from llm_compileforge_b200 import _lib, ops
+
+    g = gen(40)
+    x, w, v, b = make(g, 2, 30, 128), make(g, 128, 96, std=0.1), make(g, 128, 96, std=0.1), make(g, 96)
+    r, flat = make(g, 2, 30, 96), make(g, 60, 128)
+    we, ve, be = make(g, 4, 128, 72, std=0.1), make(g, 72, 4, 128).permute(1, 2, 0), make(g, 4, 72)
+    offsets, index = offsets_of([10, 0, 45, 5]), torch.randint(0, 60, (60,), generator=g, device="cuda", dtype=torch.int32)
+    logits = make(g, 300, 12, dtype=F32)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def every():
+        route = ops.moe_route(logits, 3, renormalize=False)
+        y = make(gen(41), 900, 64)
+        out, out2 = torch.zeros(60, 96, dtype=F32, device="cuda"), torch.zeros(300, 64, dtype=BF16, device="cuda")
+        grouped_out = torch.zeros(60, 72, dtype=BF16, device="cuda")
+        return [ops.fused_linear(x, w, b, activation="silu", up_weight=v, up_bias=b, residual=r, status=status), ops.fused_linear(flat, w, out=out),
+                ops.fused_linear(x, w, out_dtype=F32), ops.fused_linear(flat, w.t().contiguous().t(), b),
+                ops.grouped_linear(flat, we, offsets, be, activation="gelu", row_index=index, status=status), ops.grouped_linear(flat, ve, offsets, up_weight=ve),
+                ops.grouped_linear(flat, we, offsets, out=grouped_out), ops.grouped_linear(flat, we, offsets, out_dtype=F32), *route,
+                ops.moe_combine(y, route.positions, route.weights, residual=out2, out=out2, status=status), out, grouped_out]
+
+    quick = every()
+    assert _lib.calls is not _lib._NoCalls, "the extension module is not built"
+    monkeypatch.setattr(_lib, "calls", _lib._NoCalls)
+    plain = every()
+    assert len(quick) == len(plain)
+    for a, c in zip(quick, plain):
+        assert a.dtype == c.dtype and a.shape == c.shape and a.is_contiguous() == c.is_contiguous() and torch.equal(a, c)
+    assert status.item() == 0
+
+
+def test_refusals_of_cuda_operands():
+    """Bad calls with tensors where they belong: refused before a launch, the results' memory untouched."""
+    from llm_compileforge_b200 import ops
+
+    z = lambda *s, dtype=BF16: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
+    i = lambda *s: z(*s, dtype=torch.int32)  # noqa: E731
+    x, w, we = z(4, 8), z(8, 16), z(2, 8, 16)
+    bad = [
+        lambda: ops.fused_linear(x, z(9, 16)), lambda: ops.fused_linear(x, z(8, 16, dtype=F16)), lambda: ops.fused_linear(x, z(8, 16, 1)),
+        lambda: ops.fused_linear(x, w, z(15)), lambda: ops.fused_linear(x, w, z(16, dtype=F32)), lambda: ops.fused_linear(x, w, z(32)[::2]),
+        lambda: ops.fused_linear(x, w, up_bias=z(16)), lambda: ops.fused_linear(x, w, up_weight=z(8, 8)), lambda: ops.fused_linear(x, w, up_weight=z(16, 8).t()),
+        lambda: ops.fused_linear(x, w, residual=z(4, 15)), lambda: ops.fused_linear(x, w, residual=z(2, 2, 16)), lambda: ops.fused_linear(x, w, residual=z(4, 16, dtype=F32)),
+        lambda: ops.fused_linear(x, w, out=z(5, 16)), lambda: ops.fused_linear(x, w, out=z(4, 16, dtype=F16)), lambda: ops.fused_linear(x, w, out=z(16, 4).t()),
+        lambda: ops.fused_linear(x, w, out=z(1, 16).expand(4, 16)), lambda: ops.fused_linear(x, w, activation="SILU"), lambda: ops.fused_linear(x, w, activation=["silu"]),
+        lambda: ops.fused_linear(x, w, status=z(1, dtype=torch.int64)), lambda: ops.fused_linear(x, w.cpu()), lambda: ops.fused_linear(x.cpu(), w),
+        lambda: ops.fused_linear(x.double(), w.double()), lambda: ops.fused_linear(x, z(8, 32)[:, ::2]), lambda: ops.fused_linear(x, w, out_dtype=F16),
+        lambda: ops.grouped_linear(x, we, i(4)), lambda: ops.grouped_linear(x, we, i(3).long()), lambda: ops.grouped_linear(x, we, i(6)[::2]),
+        lambda: ops.grouped_linear(x, we, i(3), row_index=i(4).long()), lambda: ops.grouped_linear(x, we, i(3), row_index=i(8)[::2]),
+        lambda: ops.grouped_linear(x, we, i(3), z(2, 15)), lambda: ops.grouped_linear(x, we, i(3), z(16)), lambda: ops.grouped_linear(x, we, i(3), out=z(5, 16)),
+        lambda: ops.grouped_linear(x, we, i(3), row_index=i(6), out=z(4, 16)), lambda: ops.grouped_linear(x[:0], we, i(3), row_index=i(4)),
+        lambda: ops.grouped_linear(x, z(1025, 8, 8), i(1026)), lambda: ops.grouped_linear(x, we, i(3).cpu()), lambda: ops.grouped_linear(x, we, i(3), workspace=z(9).cpu()),
+        lambda: ops.moe_route(z(4, 8), 9), lambda: ops.moe_route(z(4, 8), 0), lambda: ops.moe_route(z(4, 64), 33), lambda: ops.moe_route(z(4, 8), -1),
+        lambda: ops.moe_route(z(4, 2000), 2), lambda: ops.moe_route(z(4, 8, dtype=torch.float64), 2), lambda: ops.moe_route(z(8), 1), lambda: ops.moe_route(i(4, 8), 1),
+        lambda: ops.moe_combine(x, i(3, 2), z(3, 2)), lambda: ops.moe_combine(x, i(3, 2).long(), z(3, 2, dtype=F32)), lambda: ops.moe_combine(x, i(3, 33), z(3, 33, dtype=F32)),
+        lambda: ops.moe_combine(x, i(3, 2), z(2, 2, dtype=F32)), lambda: ops.moe_combine(x, i(3, 2), z(3, 2, dtype=F32), residual=z(3, 9)),
+        lambda: ops.moe_combine(x, i(3, 2), z(3, 2, dtype=F32), residual=z(3, 8, dtype=F16)), lambda: ops.moe_combine(x, i(3, 2), z(3, 2, dtype=F32), out=z(1, 8).expand(3, 8)),
+        lambda: ops.moe_combine(x, i(3, 2), z(2, 3, dtype=F32).t()),
+    ]
+    for n, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {n} was not refused")
+    torch.cuda.synchronize()
