@@ -1,7 +1,7 @@
 """Per-kernel measurements for the hot path's other kernels (one JSON line each).
 
     python -m llm_compileforge_b200.kernel_bench [--iters 20] [--chunk-tokens 0] \
-        [--only prefill,prefill_fp8,norm_matmul,append,norm,decode_c2,decode_c3,shared_prefix]
+        [--only prefill,prefill_fp8,norm_matmul,append,norm,decode_c2,decode_c3,shared_prefix,linear,routed]
 
 ``bench.py`` at the repository root reports the headline decode metric; this
 module times the remaining kernels on their configurations with CUDA events
@@ -239,6 +239,58 @@ def bench_shared_prefix(dev, iters, n_requests=32):
             "equivalent_gbs": plain_bytes / (ms_shared / 1e3) / 1e9, "timing": "CUDA graph replay, L2 flushed"}
 
 
+def _linear_line(name, workload, ms, n_bytes, flops):
+    pk = _peaks()
+    floor = max(n_bytes / (pk["hbm_gbs"] * 1e6), flops / (pk["bf16_tflops"] * 1e9))
+    return {"kernel": name, "workload": workload, "ms": ms, "achieved_gbs": n_bytes / ms / 1e6, "achieved_tflops": flops / ms / 1e9, "floor_ms": floor,
+            "frac": floor / ms, "peaks": pk["kind"], "timing": "CUDA graph replay, L2 flushed"}
+
+
+def bench_linear(dev, iters):
+    """fused_linear from one token to a prefill batch, Llama-3-8B-shaped widths."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    r = lambda *s, std=1.0: (torch.randn(s, generator=g, device=dev) * std).to(torch.bfloat16)  # noqa: E731
+    for rows, k, n, gated in ((1, 4096, 4096, False), (64, 4096, 14336, True), (1024, 4096, 4096, False), (8192, 4096, 14336, True)):
+        x, w, v = r(rows, k), r(k, n, std=k ** -0.5), r(k, n, std=k ** -0.5) if gated else None
+        res = None if gated else r(rows, n)
+        out = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
+        ms = time_ms_graph(lambda: ops.fused_linear(x, w, activation="silu" if gated else "none", up_weight=v, residual=res, out=out), iters, flush=L2Flush(dev))
+        mats = 2 if gated else 1
+        yield _linear_line("fused_linear", f"[{rows}, {k}] x [{k}, {n}]" + (" gated silu" if gated else " + residual") + ", bf16", ms,
+                           2 * (rows * k + mats * k * n + rows * n * (1 if gated else 2)), 2.0 * mats * rows * k * n)
+
+
+def bench_routed(dev, iters):
+    """One routed feed-forward layer (router, gated experts, combine) of a decode and of a prefill batch, and its parts."""
+    g = torch.Generator(device=dev).manual_seed(2)
+    r = lambda *s, std=1.0: (torch.randn(s, generator=g, device=dev) * std).to(torch.bfloat16)  # noqa: E731
+    experts, top_k, hidden, inner = 32, 4, 4096, 1792
+    router, w1, w3, w2 = r(hidden, experts, std=0.02), r(experts, hidden, inner, std=0.02), r(experts, hidden, inner, std=0.02), r(experts, inner, hidden, std=0.02)
+    for tokens in (32, 4096):
+        x = r(tokens, hidden)
+        logits = ops.fused_linear(x, router, out_dtype=torch.float32)
+        route = ops.moe_route(logits, top_k)
+        first = lambda: ops.grouped_linear(x, w1, route.group_offsets, activation="silu", up_weight=w3, row_index=route.token_rows)  # noqa: E731
+        h = first()
+        second = lambda: ops.grouped_linear(h, w2, route.group_offsets)  # noqa: E731
+        y = second()
+        last = lambda: ops.moe_combine(y, route.positions, route.weights, residual=x)  # noqa: E731
+
+        def layer():
+            t = ops.moe_route(ops.fused_linear(x, router, out_dtype=torch.float32), top_k)
+            a = ops.grouped_linear(x, w1, t.group_offsets, activation="silu", up_weight=w3, row_index=t.token_rows)
+            return ops.moe_combine(ops.grouped_linear(a, w2, t.group_offsets), t.positions, t.weights, residual=x)
+
+        rows, used = tokens * top_k, int((route.group_offsets.diff() > 0).sum())
+        parts = (("moe_route", lambda: ops.moe_route(logits, top_k), 4 * tokens * experts + 16 * rows, 0.0),
+                 ("grouped_linear, gated, rows by index", first, 2 * (tokens * hidden + 2 * used * hidden * inner + rows * inner), 4.0 * rows * hidden * inner),
+                 ("grouped_linear", second, 2 * (rows * inner + used * hidden * inner + rows * hidden), 2.0 * rows * hidden * inner),
+                 ("moe_combine", last, 2 * hidden * (rows + 2 * tokens), 2.0 * rows * hidden))
+        total_bytes, total_flops = sum(p[2] for p in parts), sum(p[3] for p in parts)
+        for name, fn, n_bytes, flops in (*parts, ("routed layer", layer, total_bytes, total_flops)):
+            yield _linear_line(name, f"{tokens} tokens, top {top_k} of {experts} experts of [{hidden}, {inner}], bf16", time_ms_graph(fn, iters, flush=L2Flush(dev)), n_bytes, flops)
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default="prefill,norm_matmul,append,norm,decode_c2,decode_c3,shared_prefix")
@@ -266,6 +318,12 @@ def main() -> None:
     if "shared_prefix" in which:
         for n in (32, 128, 512):
             print(json.dumps(bench_shared_prefix(dev, args.iters, n)), flush=True)
+    if "linear" in which:
+        for line in bench_linear(dev, args.iters):
+            print(json.dumps(line), flush=True)
+    if "routed" in which:
+        for line in bench_routed(dev, args.iters):
+            print(json.dumps(line), flush=True)
     if "decode_c2" in which:
         print(json.dumps(bench_decode(dev, args.iters, wl.C2, args.chunk_tokens)), flush=True)
     if "decode_c3" in which:
