@@ -467,7 +467,7 @@ enum { SFB_WEIGHT_KN = 0, /* [.., K, N], N contiguous */ SFB_WEIGHT_NK = 1 /* [.
  *   x [M, K]  weight [K, N] or [N, K] (weight_layout)  bias [N] or NULL
  *   up_weight (V) like weight, or NULL: then the second factor is left out;  up_bias [N] or NULL (needs up_weight)
  *   residual [M, N] in out_dtype or NULL; it may be `out` itself
- *   out [M, N] in out_dtype: dtype or F32.  dtype: F32, BF16, F16
+ *   out [M, N] in out_dtype: dtype or F32; it shares memory with no other operand.  dtype: F32, BF16, F16
  * Products and sums in fp32 (16-bit products are exact there), one rounding of the result.  bf16 / fp16 operands whose
  * bases and row strides are multiples of 16 bytes run on the tensor cores; every other type, alignment and stride on
  * the CUDA cores. */
@@ -479,7 +479,7 @@ SFB_API int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const 
  * i = row_index[r], or r without a row_index.
  *   x [X, K]  weight, up_weight [E, K, N] or [E, N, K]  bias, up_bias [E, N] or NULL
  *   group_offsets int32 [E + 1], read on the device: not decreasing, within 0 .. R; groups may be empty
- *   row_index int32 [R] or NULL  out [R, N]
+ *   row_index int32 [R] or NULL  out [R, N], sharing memory with no operand
  * Rows of out outside every group are left as they were.  E <= 1024.  Offsets that leave 0 .. R are clamped, one below
  * an offset before it counts as that one, and a row index outside 0 .. X-1 reads row 0; each sets
  * SFB_STATUS_BAD_ROW_INDEX.
@@ -511,7 +511,8 @@ SFB_API int sfb_moe_route(const SFBTensor* logits, SFBTensor* expert_ids, SFBTen
                           SFBTensor* positions, int dtype, int renormalize, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* out[t, :] = sum over j of weights[t, j] y[positions[t, j], :]  + residual[t, :]
- *   y [R, H]  positions int32, weights float32 [T, k], k <= 32  residual, out [T, H] (residual may be NULL or `out` itself)
+ *   y [R, H]  positions int32, weights float32 [T, k], k <= 32  residual, out [T, H] (residual may be NULL or `out` itself; `out`
+ *   shares memory with nothing else)
  * dtype F32, BF16 or F16 for y, residual and out; fp32 sums in the order of j, one rounding.  Position -1 adds nothing;
  * any other position outside 0 .. R-1 adds nothing either and sets SFB_STATUS_BAD_ROW_INDEX. */
 SFB_API int sfb_moe_combine(const SFBTensor* y, const SFBTensor* positions, const SFBTensor* weights, const SFBTensor* residual, SFBTensor* out,

@@ -25,6 +25,33 @@ int index_view(const SFBTensor* t, const char* what, int rank, View* v) {
     return SFB_OK;
 }
 
+// Whether rows [rows][width bytes], `stride` bytes apart, share memory with others.  Exact for equal strides (column slices of
+// one buffer) and where either is one block of memory; two interleaved patterns of different strides are left to the caller.
+struct Rows {
+    const char* base;
+    int64_t rows, stride, width;
+    Rows(const void* p, int64_t n, int64_t stride_elements, int64_t columns, int elem)
+        : base(static_cast<const char*>(p)), rows(n), stride(n > 1 ? stride_elements * elem : columns * elem), width(columns * elem) {}
+    const char* end() const { return base + (rows - 1) * stride + width; }
+};
+bool share_memory(const Rows& a, const Rows& b) {
+    if (a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1 || a.end() <= b.base || b.end() <= a.base) return false;
+    for (int i = 0; i < 2; ++i) {
+        const Rows &block = i ? b : a, &other = i ? a : b;
+        if (block.stride > block.width) continue;
+        if (other.stride <= 0) return true;
+        // the first row of `other` that ends behind the block's start
+        const int64_t before = block.base - other.base - other.width, first = before < 0 ? 0 : before / other.stride + 1;
+        return first < other.rows && other.base + first * other.stride < block.end();
+    }
+    if (a.stride != b.stride) return false;
+    const int64_t apart = ((b.base - a.base) % a.stride + a.stride) % a.stride;
+    return apart < a.width || apart + b.width > a.stride;
+}
+
+// Row and column numbers are 32-bit, those of a tile's end and of a grid stride further on too.
+constexpr int64_t kMostRows = 0x7fff0000LL;
+
 // Fills the parts that the dense and the grouped product have in common.
 int linear_views(const char* op, const SFBTensor* x, const SFBTensor* weight, const SFBTensor* bias, const SFBTensor* up_weight,
                  const SFBTensor* up_bias, SFBTensor* out, bool grouped, int layout, int dtype, int out_dtype, int activation, LinearArgs* a) {
@@ -68,7 +95,7 @@ int linear_views(const char* op, const SFBTensor* x, const SFBTensor* weight, co
     a->dtype = dtype;
     a->out_dtype = out_dtype;
     a->act = activation;
-    const int64_t most = 0x7fffffffLL;
+    const int64_t most = kMostRows;
     if (a->rows > most || a->x_rows > most || a->K > most || a->N > most) return fail(SFB_ERR_UNSUPPORTED, "%s: dimension too large", op);
     return SFB_OK;
 }
@@ -99,6 +126,11 @@ int sfb_fused_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTenso
     }
     if (a.rows == 0 || a.N == 0) return SFB_OK;
     if (a.K == 0) return fail(SFB_ERR_INVALID_ARG, "fused_linear: K is zero");
+    const Rows o(a.out, a.rows, a.out_stride, a.N, dtype_size(out_dtype));
+    if (share_memory(o, Rows(a.x, a.x_rows, a.x_stride, a.K, dtype_size(dtype)))) return fail(SFB_ERR_INVALID_ARG, "fused_linear: out shares memory with x");
+    if (a.residual && !(a.residual == a.out && (a.rows == 1 || a.res_stride == a.out_stride)) &&
+        share_memory(o, Rows(a.residual, a.rows, a.res_stride, a.N, dtype_size(out_dtype))))
+        return fail(SFB_ERR_INVALID_ARG, "fused_linear: out shares memory with the residual, but is not the residual");
     a.status = status;
     return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
@@ -130,6 +162,8 @@ int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTen
     }
     if (a.rows == 0 || a.N == 0) return SFB_OK;
     if (a.K == 0) return fail(SFB_ERR_INVALID_ARG, "grouped_linear: K is zero");
+    if (share_memory(Rows(a.out, a.rows, a.out_stride, a.N, dtype_size(out_dtype)), Rows(a.x, a.x_rows, a.x_stride, a.K, dtype_size(dtype))))
+        return fail(SFB_ERR_INVALID_ARG, "grouped_linear: out shares memory with x");
     a.workspace = workspace;
     a.workspace_bytes = workspace ? workspace_bytes : 0;
     a.status = status;
@@ -137,7 +171,7 @@ int sfb_grouped_linear(const SFBTensor* x, const SFBTensor* weight, const SFBTen
 }
 
 int sfb_linear_plan(int64_t rows, int64_t K, int64_t N, int64_t groups, int gated, int indexed, int has_workspace, int sms, int32_t* plan6) {
-    if (rows < 1 || K < 1 || N < 1 || groups < 0 || groups > kMaxGroups || sms < 1 || !plan6) return fail(SFB_ERR_INVALID_ARG, "linear_plan: bad argument");
+    if (rows < 1 || K < 1 || N < 1 || rows > kMostRows || K > kMostRows || N > kMostRows || groups < 0 || groups > kMaxGroups || sms < 1 || !plan6) return fail(SFB_ERR_INVALID_ARG, "linear_plan: bad argument");
     const LinearPlan p = plan_linear(rows, K, N, groups ? groups : 1, groups > 0, gated != 0, groups > 0 && indexed, has_workspace != 0, sms);
     plan6[0] = p.tokens; plan6[1] = p.pair; plan6[2] = p.split; plan6[3] = p.order; plan6[4] = p.blocks_an_sm; plan6[5] = (int32_t)p.feat_tiles;
     return SFB_OK;
@@ -211,6 +245,10 @@ int sfb_moe_combine(const SFBTensor* y, const SFBTensor* positions, const SFBTen
         a.res_stride = vr.stride[2];
     }
     if (T == 0 || H == 0) return SFB_OK;
+    const Rows o(vo.base, T, vo.stride[2], H, e);
+    if (share_memory(o, Rows(vy.base, vy.size[2], vy.stride[2], H, e))) return fail(SFB_ERR_INVALID_ARG, "moe_combine: out shares memory with y");
+    if (residual && !(a.residual == vo.base && (T == 1 || a.res_stride == vo.stride[2])) && share_memory(o, Rows(vr.base, T, vr.stride[2], H, e)))
+        return fail(SFB_ERR_INVALID_ARG, "moe_combine: out shares memory with the residual, but is not the residual");
     a.y = vy.base; a.y_stride = vy.stride[2]; a.y_rows = vy.size[2];
     a.positions = reinterpret_cast<const int32_t*>(vp.base); a.pos_stride = vp.stride[2];
     a.weights = reinterpret_cast<const float*>(vw.base); a.weight_stride = vw.stride[2];

@@ -34,7 +34,6 @@
 #include <cmath>
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "linear.cuh"
 
@@ -439,6 +438,11 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                     if (++s == stages) { s = 0; ephase ^= 1; }
                 }
             }
+            // the leader's commits arrive in both blocks: none may still be under way when this one leaves
+            for (uint32_t i = 0; PAIR && i < stages && !timed_out; ++i) {
+                timed_out = !mbar_wait(bar(B_EMPTY + s), ephase);
+                if (++s == stages) { s = 0; ephase ^= 1; }
+            }
         }
     } else if (warp == kRowWarp) {
         // =========================== rows' producer ===========================
@@ -721,6 +725,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             int m = rank * kEpilogueWarps + warp;
             float r[4] = {};
             if (m < tile.rows) residual_of(tile.row0 + m, r);
+            __syncwarp();
             cluster_sync();  // (1)
             for (; there && m < tile.rows; m += split * kEpilogueWarps) {
                 float q[1][4] = {}, part[kMaxSplit][4];
@@ -846,11 +851,13 @@ bool rows_for_tma(const void* base, int64_t inner, int64_t rows, int64_t stride,
 // device and size.
 int resident_clusters(const void* kernel, int size, int dev, int sms) {
     struct Known { const void* kernel; int size, dev, clusters; };
+    constexpr int kMost = 1024;  // kernels x sizes x devices of any machine; asked again beyond
     static std::mutex mu;
-    static std::vector<Known> known;
+    static Known known[kMost];
+    static int count = 0;
     std::lock_guard<std::mutex> lock(mu);
-    for (const Known& k : known)
-        if (k.kernel == kernel && k.size == size && k.dev == dev) return k.clusters;
+    for (int i = 0; i < count; ++i)
+        if (known[i].kernel == kernel && known[i].size == size && known[i].dev == dev) return known[i].clusters;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -861,7 +868,7 @@ int resident_clusters(const void* kernel, int size, int dev, int sms) {
     if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
     cudaGetLastError();  // a refusal only means "not available"
     clusters = std::max(0, std::min(clusters, sms / size));
-    known.push_back({kernel, size, dev, clusters});
+    if (count < kMost) known[count++] = {kernel, size, dev, clusters};
     return clusters;
 }
 
@@ -885,8 +892,8 @@ int launch_tiles(const CUtensorMap* maps, TileArgs a, int64_t units, bool shared
 
 // Every candidate shape is priced in clocks: a start and the last tile's epilogue, and between them the longer of the weights'
 // way from HBM (3400 bytes a clock) and the rounds of tiles on the busiest SM x their K steps x a step.  A step takes the longest
-// of its MMAs (2 clocks a token column, with what lies between them 2.3 for a pair), its operands' way into shared memory (72 bytes a clock an SM), the issuing thread's
-// chain (380 clocks with two steps a stage, 600 with one) and the row gathers (62 clocks for four rows); two blocks an SM share
+// of its MMAs (2 clocks a token column, with what lies between them 2.3 for a
+// pair), its operands' way into shared memory (72 bytes a clock an SM), the issuing thread's chain (380 clocks with two steps a stage, 600 with one) and the row gathers (62 clocks for four rows); two blocks an SM share
 // the first two.  A split launches a cluster for every tile and exchanges sums at its end; how many clusters run at once goes
 // by the smallest of the eight groups of SMs that a cluster must lie in.
 static LinearPlan price_shapes(int64_t rows, int64_t K, int64_t N, int64_t groups, bool grouped, bool gated, bool indexed, bool ordered, int sms) {

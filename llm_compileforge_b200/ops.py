@@ -8,6 +8,7 @@ dict-based signatures of the reference's ``kernels`` package are in
 
 from __future__ import annotations
 
+import operator
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -502,6 +503,14 @@ def _done(got):
     return got
 
 
+def _out_type(what: str, dtype: torch.dtype, out: torch.Tensor | None, out_dtype: torch.dtype | None) -> torch.dtype:
+    if out is None:
+        return out_dtype or dtype
+    if out_dtype not in (None, out.dtype):
+        raise ValueError(f"{what}: out is {out.dtype}, out_dtype {out_dtype}")
+    return out.dtype
+
+
 def _activation(what: str, name: str) -> int:
     try:
         return ACTIVATIONS[name]
@@ -516,7 +525,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     optional.  ``x [..., K]``, ``weight`` and ``up_weight`` ``[K, N]`` with either dimension contiguous (a checkpoint's
     ``[N, K]`` matrix goes in as its ``.t()`` view), ``residual [..., N]`` in the result's type.  ``activation``: one of
     :data:`ACTIVATIONS`.  The result has ``x``'s type, or float32 with ``out_dtype=torch.float32``; ``out`` may be the residual
-    itself.  fp32 accumulation, one rounding.  bf16 / fp16 operands whose rows are 16-byte aligned run on the tensor
+    itself, but share memory with no other operand.  fp32 accumulation, one rounding.  bf16 / fp16 operands whose rows are 16-byte aligned run on the tensor
     cores, all others on the CUDA cores.  ``status`` (int32, device) collects status bits."""
     if type(activation) is str and (out_dtype is None or out_dtype is torch.float32):
         got = _quick("linear")(x, weight, bias, up_weight, up_bias, residual, out, status, ACTIVATIONS.get(activation, -1), out_dtype is not None)
@@ -527,7 +536,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"fused_linear: x [..., K] and weight [K, N], got {tuple(xs)} and {tuple(ws)}")
     k, n = ws
     act = _activation("fused_linear", activation)
-    odt = out.dtype if out is not None else out_dtype or dtype
+    odt = _out_type("fused_linear", dtype, out, out_dtype)
     _same_type("fused_linear", dtype, "weight bias up_weight up_bias", weight, bias, up_weight, up_bias)
     if k == 0:
         raise ValueError("fused_linear: K is zero")
@@ -584,9 +593,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     ``[E + 1]``, read on the device, groups may be empty) is ``act(x[i] @ weight[e] + bias[e]) * (x[i] @ up_weight[e] + up_bias[e])``
     with ``i = row_index[r]`` (int32, one entry per row of the result) or ``i = r`` without one.  ``weight`` and ``up_weight``
     ``[E, K, N]`` with either of the last two dimensions contiguous, biases ``[E, N]``.  Rows outside every group are left as
-    they were (in a fresh result: undefined).  ``workspace`` (uint8, :func:`grouped_linear_workspace_bytes`; allocated when
-    missing) holds the rows of ``x`` in the order of ``row_index`` where groups have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or
-    indices outside their range."""
+    they were (in a fresh result: undefined).  ``out`` shares memory with no operand.  ``workspace`` (uint8,
+    :func:`grouped_linear_workspace_bytes`; allocated when missing) holds the rows of ``x`` in the order of ``row_index`` where groups
+    have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or indices outside their range."""
     if type(activation) is str and (out_dtype is None or out_dtype is torch.float32):
         got = _quick("grouped")(x, weight, group_offsets, bias, up_weight, up_bias, row_index, out, workspace, status, ACTIVATIONS.get(activation, -1),
                                 out_dtype is not None)
@@ -597,7 +606,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
         raise ValueError(f"grouped_linear: x [X, K] and weight [E, K, N], got {tuple(xs)} and {tuple(ws)}")
     e, k, n = ws
     act = _activation("grouped_linear", activation)
-    odt = out.dtype if out is not None else out_dtype or dtype
+    odt = _out_type("grouped_linear", dtype, out, out_dtype)
     _same_type("grouped_linear", dtype, "weight bias up_weight up_bias", weight, bias, up_weight, up_bias)
     _same_type("grouped_linear", torch.int32, "group_offsets row_index", group_offsets, row_index)
     if x.stride(1) != 1 and k > 1:
@@ -662,7 +671,7 @@ def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, wor
         raise ValueError(f"moe_route: logits [T, E], got {tuple(ls)}")
     if logits.stride(1) != 1 and ls[1] > 1:
         logits = logits.contiguous()
-    (t, e), k, dev = ls, int(top_k), logits.get_device()
+    (t, e), k, dev = ls, operator.index(top_k), logits.get_device()
     if k < 1 or k > min(e, 32):
         raise ValueError(f"moe_route: top_k {k} outside 1 .. min(experts, 32)")
     results = logits.new_empty((4, t, k), dtype=torch.int32)  # one allocation for the four of that size
@@ -689,7 +698,8 @@ def moe_combine(y: torch.Tensor, positions: torch.Tensor, weights: torch.Tensor,
                 out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """``out[t] = sum_j weights[t, j] * y[positions[t, j]] (+ residual[t])``: every token's experts' rows (``y [R, H]``, the last
     :func:`grouped_linear`'s result) back to the token; ``positions`` int32 and ``weights`` float32 ``[T, top_k]`` are
-    :func:`moe_route`'s.  A position of -1 adds nothing.  fp32 sums in the order of j, one rounding; ``out`` may be the residual."""
+    :func:`moe_route`'s.  A position of -1 adds nothing.  fp32 sums in the order of j, one rounding; ``out`` may be the residual, but share memory
+    with nothing else."""
     got = _quick("combine")(y, positions, weights, residual, out, status)
     if got is not None:
         return _done(got)

@@ -1,5 +1,7 @@
 """Refusals of the feed-forward operators, without a GPU: every bad call ends in ValueError before a launch."""
 
+import random
+
 import pytest
 import torch
 
@@ -88,6 +90,51 @@ def test_library_refuses_bad_descriptors():
         lin(*args)
         assert text in _lib.load().sfb_last_error().decode()
     assert lin(d((0, 8), 2), w, None, None, None, None, d((0, 16), 2)) == _lib.SFB_OK  # nothing to do
+
+
+def rows_desc(ptr, rows, columns, stride):
+    return _fake_desc((rows, columns), 2, ptr=ptr, strides=[stride, 1])
+
+
+def test_shared_memory_is_refused_where_it_is_shared():
+    """out over x or over part of the residual, against the sets of their elements."""
+    g = random.Random(4)
+    refused = allowed = 0
+    for case in range(400):
+        rows, k, n = g.choice([1, 2, 5]), 8, g.choice([8, 16])
+        stride = g.choice([16, 24, 40])
+        xs = g.choice([stride, stride, k, 0, 4])
+        x0, o0 = 0x10000, 0x10000 + 2 * g.randrange(-100, 100)
+        x = {x0 + 2 * (r * xs + c) for r in range(rows) for c in range(k)}
+        o = {o0 + 2 * (r * stride + c) for r in range(rows) for c in range(n)}
+        if stride < n or (xs != stride and xs > k and stride > n):
+            continue
+        rc = lin(rows_desc(x0, rows, k, xs), _fake_desc((k, n), 2, ptr=0x900000), None, None, None, None, rows_desc(o0, rows, n, stride))
+        assert rc != _lib.SFB_OK  # no device here: what passes the checks fails at the launch
+        assert (rc == _lib.SFB_ERR_INVALID_ARG) == bool(x & o), (rows, k, n, stride, xs, o0 - x0)
+        refused, allowed = refused + bool(x & o), allowed + (not x & o)
+    assert refused > 50 and allowed > 50
+    x, w, o = rows_desc(0x10000, 4, 8, 8), _fake_desc((8, 16), 2, ptr=0x20000), rows_desc(0x30000, 4, 16, 16)
+    assert lin(x, w, None, None, None, o, o) != _lib.SFB_ERR_INVALID_ARG  # the residual itself
+    assert lin(x, w, None, None, None, rows_desc(0x30020, 4, 16, 16), o) == _lib.SFB_ERR_INVALID_ARG  # a row further on
+    assert lin(x, w, None, None, None, rows_desc(0x30000, 4, 16, 0), o) == _lib.SFB_ERR_INVALID_ARG  # its first row for all
+    assert "residual" in _lib.load().sfb_last_error().decode()
+
+
+def test_sizes_beyond_32_bit_rows_are_refused():
+    n = 2 ** 31 - 1
+    assert lin(rows_desc(0x10000, n, 8, 0), _fake_desc((8, 8), 2, ptr=0x20000), None, None, None, None, rows_desc(1 << 40, n, 8, 8)) == _lib.SFB_ERR_UNSUPPORTED
+    with pytest.raises(ValueError):
+        ops.linear_plan(n, 8, 8)
+
+
+def test_types_of_out_and_of_top_k():
+    with pytest.raises(ValueError, match="out_dtype"):
+        ops.fused_linear(t(4, 8), t(8, 8), out=t(4, 8), out_dtype=torch.float32)
+    with pytest.raises(ValueError, match="out_dtype"):
+        ops.grouped_linear(t(4, 8), t(2, 8, 8), i32(3), out=t(4, 8), out_dtype=torch.float32)
+    with pytest.raises(TypeError):
+        ops.moe_route(t(4, 8), 2.5)
 
 
 def test_route_workspace_query():

@@ -643,6 +643,85 @@ def test_results_behind_other_kernels():
         assert torch.equal(h, want)
 
 
+def test_offsets_past_32_bits():
+    """Rows, experts and results 2^26 elements apart, so that the last lie more than 2^31 elements behind the first."""
+    from llm_compileforge_b200 import ops
+
+    g, rows, apart, k, n = gen(50), 40, 2 ** 26, 128, 72
+    buffer = torch.empty(rows * apart, dtype=BF16, device="cuda")
+
+    def far(first, columns, fill=None):
+        view = buffer.as_strided((rows, columns), (apart, 1), first)
+        if fill is not None:
+            view.copy_(fill)
+        return view
+
+    for odd in (0, 1):  # 1: bases that only the CUDA cores take
+        x, r = far(odd, k, make(g, rows, k)), far(1024 + odd, n, make(g, rows, n))
+        experts = buffer.as_strided((rows, k, n), (apart, n, 1), 4096)
+        experts.copy_(make(g, rows, k, n, std=k ** -0.5))
+        out = far(2048 + odd, n)
+        want, tol = linear64(x, experts[-1], r=r)
+        ops.fused_linear(x, experts[-1], residual=r, out=out)
+        assert_rounded(out, want, tol, "dense")
+        offsets, index = torch.arange(rows + 1, dtype=torch.int32, device="cuda"), torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda")
+        ops.grouped_linear(x, experts, offsets, row_index=index, out=out)
+        for e in (0, 20, rows - 1):
+            want, tol = linear64(x[rows - 1 - e:rows - e], experts[e])
+            assert_rounded(out[e:e + 1], want, tol, f"expert {e}")
+        positions, weights = torch.stack([index, index], 1).contiguous(), torch.rand(rows, 2, generator=g, device="cuda")
+        ops.moe_combine(x, positions, weights, residual=far(512 + odd, k, make(g, rows, k)), out=far(6144 * 4 + odd, k))
+        near = ops.moe_combine(x.contiguous(), positions, weights, residual=far(512 + odd, k).contiguous())
+        assert torch.equal(far(6144 * 4 + odd, k), near)
+        got, want = ops.moe_route(x, 4), ops.moe_route(x.contiguous(), 4)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("rows", [3, 200, 700])
+def test_captured_behind_copies_joins_and_at_the_start(rows):
+    """Calls as a graph's first node, behind a copy and a fill, beside one another and behind a join of two streams."""
+    from llm_compileforge_b200 import ops
+
+    g = gen(51)
+    x, w, v = make(g, rows, 256), make(g, 256, 256, std=0.06), make(g, 256, 256, std=0.06)
+    index, offsets = torch.randperm(rows, generator=g, device="cuda").int(), offsets_of([rows // 3, rows - rows // 3])
+    both = torch.stack([w, v])
+    side = torch.cuda.Stream()
+
+    def work():
+        here = torch.cuda.current_stream()
+        a = ops.fused_linear(x, w)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = ops.fused_linear(a, v, activation="silu")
+            b2 = ops.grouped_linear(b, both, offsets, row_index=index)
+        c = torch.empty_like(a).copy_(a)
+        d = ops.fused_linear(c, v)
+        here.wait_stream(side)
+        e = ops.fused_linear(d, w, residual=b2)
+        f = torch.zeros_like(e)
+        ops.fused_linear(e, v, residual=f, out=f)
+        route = ops.moe_route(f[:, :16], 2)
+        y = ops.moe_combine(f, route.positions.clamp(max=rows - 1), route.weights, residual=e)
+        return [a, b, b2, d, e, f, *route, y]
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for _ in range(3):
+        x.copy_(make(g, rows, 256))
+        want = [t.clone() for t in work()]
+        torch.cuda.synchronize()
+        for t in held:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, (a, b) in enumerate(zip(held, want)):
+            assert torch.equal(a, b), n
+
+
 # ── the two ways from Python into the library ────────────────────────────────
 def test_both_ways_into_the_library_agree(monkeypatch):
     from llm_compileforge_b200 import _lib, ops
