@@ -104,6 +104,7 @@ struct TileArgs {
     int block;       // token tiles that run together through the feature tiles (L2 reuse of x and W)
     int act;
     bool gated, nk, out_f32, vec;
+    bool ordered;    // the kernel before this one is order_rows_kernel, and only x comes from it
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -367,7 +368,9 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == kMmaWarp) tmem_alloc<PAIR>(smem_u32(tmem_slot), 2 * kTok);
-    wait_for_previous();
+    // order_rows_kernel lets this one start when all before it has ended, so only who reads its rows waits for it, further down:
+    // the pipeline fills with weights meanwhile
+    if (!a.ordered) wait_for_previous();
     if (warp == 0) {  // the groups' rows, and the running number of token tiles
         int before = 0, top = a.offsets ? group_offset(a.offsets[0], 0, a.rows) : 0;
         bool bad = a.offsets && top != a.offsets[0];
@@ -447,6 +450,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     } else if (warp == kRowWarp) {
         // =========================== rows' producer ===========================
         // Lane j loads the j-th box, with a row index the j-th four rows.
+        if (a.ordered) wait_for_previous();
         const uint32_t full0 = leader_bar(B_FULL);
         uint32_t s = 0, ephase = 1;
         for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
@@ -781,33 +785,48 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     }
 }
 
-// Rows of x in the order of out: ordered[r, :] = x[row_index[r], :] for the rows that lie in a group.
+// Rows of x in the order of out: ordered[r, :] = x[row_index[r], :].  A warp keeps 2 KB of the rows and walks them, the index read
+// one row ahead.  Only an index that is no row needs the groups: inside one it counts as row 0 and is flagged, outside it is what
+// the router leaves behind the last row and nothing is written.  (Rows outside every group with an index that is a row are copied
+// like the others; nobody reads them.)  16384 rows of 4096 take
+// 23 us, 4096 of 1024 2.5 (a block a row, its 256 threads in step and without the index ahead: 26 and 4.7).
+constexpr int kPieceValues = 1024;
 __global__ void __launch_bounds__(256) order_rows_kernel(const uint16_t* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ row_index,
-                                                         const int32_t* __restrict__ offsets, int groups, int rows, int x_rows, int K,
+                                                         const int32_t* __restrict__ offsets, int groups, int rows, int x_rows, int K, int pieces,
                                                          uint16_t* __restrict__ ordered, int64_t ordered_stride, int* status) {
-    let_next_start();
     wait_for_previous();
-    int first = group_offset(offsets[0], 0, rows), end = first;
-    for (int e = threadIdx.x; e < groups; e += 256) end = group_offset(offsets[e + 1], end, rows);
-    __shared__ int ends[256];
-    ends[threadIdx.x] = end;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if (threadIdx.x < o) ends[threadIdx.x] = max(ends[threadIdx.x], ends[threadIdx.x + o]);
-        __syncthreads();
-    }
-    end = ends[0];
-    for (int r = first + blockIdx.x; r < end; r += gridDim.x) {
-        int i = row_index[r];
+    let_next_start();  // in this order: what the next kernel reads of others than this one is then there when it starts
+    const int lane = threadIdx.x & 31;
+    const int block = (int)blockIdx.x / pieces, p = (int)blockIdx.x - block * pieces, step = (int)gridDim.x / pieces * 8;
+    int r = block * 8 + (int)(threadIdx.x >> 5);
+    int next = r < rows ? row_index[r] : 0;
+    int first = -1, end = -1;  // of the rows inside groups, once asked for
+    for (; r < rows; r += step) {
+        int i = next;
+        if (r + step < rows) next = row_index[r + step];
         if (i < 0 || i >= x_rows) {
-            if (status && threadIdx.x == 0) atomicOr(status, SFB_STATUS_BAD_ROW_INDEX);
+            if (first < 0) {
+                first = group_offset(offsets[0], 0, rows);
+                end = first;
+                for (int e = lane; e < groups; e += 32) end = group_offset(offsets[e + 1], end, rows);
+                end = __reduce_max_sync(0xffffffffu, end);
+            }
+            if (r < first || r >= end) continue;
+            if (status && lane == 0) atomicOr(status, SFB_STATUS_BAD_ROW_INDEX);
             i = 0;
         }
         const uint16_t* src = x + (int64_t)i * x_stride;
         uint16_t* dst = ordered + (int64_t)r * ordered_stride;
-        for (int c = threadIdx.x * 8; c + 8 <= K; c += 2048) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        const int c = p * kPieceValues + lane * 8;
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j * 256 + 8 <= K) v[j] = *reinterpret_cast<const uint4*>(src + c + j * 256);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j * 256 + 8 <= K) *reinterpret_cast<uint4*>(dst + c + j * 256) = v[j];
         const int tail = K & ~7;
-        if (threadIdx.x < K - tail) dst[tail + threadIdx.x] = src[tail + threadIdx.x];
+        if (p == pieces - 1 && lane < K - tail) dst[tail + lane] = src[tail + lane];
     }
 }
 
@@ -917,7 +936,7 @@ static LinearPlan price_shapes(int64_t rows, int64_t K, int64_t N, int64_t group
         // the two overlap, but not wholly
         int64_t cost = 6000 + 25 * width + std::max(hbm, on_sm) + std::min(hbm, on_sm) / 4 + (an_sm - 1) * 1500;
         if (split > 1) cost += 3000 + 300 * split + 6000 * (rounds - 1);
-        if (order) cost += 5000 + rows * K / 1000;  // the pass that orders the rows
+        if (order) cost += 1500 + rows * K / 2000;  // the pass that orders the rows
         if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = {tokens, pair ? 1 : 0, split, order ? 1 : 0, an_sm, feat_tiles}; }
     };
     for (int order = 0; order <= (indexed && ordered ? 1 : 0); ++order) {
@@ -965,6 +984,7 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     a.rows = (int)in.rows; a.x_rows = (int)in.x_rows; a.N = (int)in.N; a.n_k = (int)ceil_div(in.K, (int64_t)kStepK); a.groups = (int)in.groups;
     a.feat_tiles = (int)plan.feat_tiles; a.split = plan.split; a.act = in.act;
     a.gated = in.up != nullptr; a.nk = nk; a.out_f32 = in.out_dtype == SFB_F32;
+    a.ordered = plan.order;
     a.block = 8;
     // rows of a box: all where they fit one (in eights); else 32, or 64 of a pair's 128, the last one bringing in some too many
     a.box_rows = !in.offsets && in.rows <= 32 ? (int)(ceil_div(in.rows, (int64_t)8) * 8) : plan.pair ? 64 : 32;
@@ -972,9 +992,10 @@ int launch_linear_tcgen05(const LinearArgs& in, cudaStream_t stream) {
     const void* x = order ? in.workspace : in.x;
     const int64_t x_rows = order ? in.rows : in.x_rows, x_row = order || x_rows == 1 ? ordered_stride : in.x_stride;
     if (order) {
-        const int rc = launch_after(order_rows_kernel, (unsigned)std::min<int64_t>(in.rows, 8 * (int64_t)sms), 256, 0, 1, stream,
-                                    static_cast<const uint16_t*>(in.x), in.x_stride, in.row_index, in.offsets, (int)in.groups, (int)in.rows,
-                                    (int)in.x_rows, (int)in.K, static_cast<uint16_t*>(in.workspace), ordered_stride, in.status);
+        const int64_t pieces = ceil_div(in.K, (int64_t)kPieceValues), blocks = pieces * std::min(ceil_div(in.rows, (int64_t)8), std::max<int64_t>(1, 8 * sms / pieces));
+        const int rc = launch_after(order_rows_kernel, (unsigned)blocks, 256, 0, 1, stream, static_cast<const uint16_t*>(in.x), in.x_stride, in.row_index,
+                                    in.offsets, (int)in.groups, (int)in.rows, (int)in.x_rows, (int)in.K, (int)pieces,
+                                    static_cast<uint16_t*>(in.workspace), ordered_stride, in.status);
         if (rc != SFB_OK) return rc;
     }
     // rows of out and residual in pieces of `cols` values where all of them start on one
