@@ -289,14 +289,47 @@ __device__ __forceinline__ bool group_any(int barrier, bool failed) {
 }
 __device__ __forceinline__ void group_sync(int barrier) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(barrier) : "memory"); }
 
-// h Phi(h).  erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + p z), for z >= 0: Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.26, absolute error 1.5e-7 - a quarter of the instructions of erfcf, which made the epilogue of
-// a [1001, 2048] x [2048, 8192] product take four times its MMAs.
-__device__ __forceinline__ float gelu_erf(float h) {
-    const float z = fabsf(h) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float q = 0.5f * poly * __expf(-z * z);  // Phi(-|h|)
-    return h * (h < 0.f ? q : 1.f - q);
+// Two fp32 operations an instruction, each rounded as by itself.
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ explicit Two(float both) : Two(both, both) {}
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(a.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return a;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v));
+    return a;
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// h Phi(h), two at a time.  Phi(-x) = exp(-x^2 / 2) R(x); on [0, 5.5] R is a polynomial of degree 11 in s = x / 2.75 - 1, the
+// minimax fit under the weight exp(-x^2 / 2) max(x, 1) (Lawson's iteration), off by 3.2e-8 under it.  Beyond, where Phi(-x) is
+// below 2e-8, R stays.  With erfcf the epilogue of a [1001, 2048] x [2048, 8192] product took four times its MMAs; with a
+// fit of one division, one value at a time, a tile's epilogue took 7.2 us, 4 of them the activation, and the product 34.3 us: now 32.2.
+__device__ __forceinline__ void gelu_erf(float& a, float& b) {
+    constexpr float c[12] = {1.307243997e-01f, -1.084814067e-01f, 8.416674024e-02f, -6.136930886e-02f, 4.155892394e-02f, -3.239707470e-02f,
+                             1.858075507e-02f, 6.317186358e-03f, 2.668746313e-02f, -1.294714752e-02f, -2.720778053e-02f, -1.661171493e-02f};
+    const Two h(a, b), s = fma2(Two(fminf(fabsf(a), 5.5f), fminf(fabsf(b), 5.5f)), Two(1.f / 2.75f), Two(-1.f));
+    Two r(c[11]);
+#pragma unroll
+    for (int i = 10; i >= 0; --i) r = fma2(r, s, Two(c[i]));
+    const float2 x = mul2(mul2(h, Two(-0.72134752f)), h).get();  // log2 e / 2
+    const Two q = mul2(r, Two(exp2_approx(x.x), exp2_approx(x.y)));  // Phi(-|h|)
+    const float2 lo = q.get(), hi = fma2(q, Two(-1.f), Two(1.f)).get();
+    const float2 y = mul2(h, Two(a < 0.f ? lo.x : hi.x, b < 0.f ? lo.y : hi.y)).get();
+    a = y.x;
+    b = y.y;
 }
 template <int W>
 __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
@@ -305,7 +338,10 @@ __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
         for (int i = 0; i < W; ++i) h[i] = f(h[i]);
     };
     if (act == SFB_ACT_SILU) each([](float v) { return __fdividef(v, 1.f + __expf(-v)); });
-    else if (act == SFB_ACT_GELU) each([](float v) { return gelu_erf(v); });
+    else if (act == SFB_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < W; i += 2) gelu_erf(h[i], h[i + 1]);
+    }
     else if (act == SFB_ACT_GELU_TANH) each([](float v) { return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v))); });
     else if (act == SFB_ACT_RELU) each([](float v) { return activate<SFB_ACT_RELU>(v); });
 }
@@ -368,9 +404,10 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == kMmaWarp) tmem_alloc<PAIR>(smem_u32(tmem_slot), 2 * kTok);
-    // order_rows_kernel lets this one start when all before it has ended, so only who reads its rows waits for it, further down:
-    // the pipeline fills with weights meanwhile
-    if (!a.ordered) wait_for_previous();
+    // The previous kernel is waited for as late as may be: here where offsets come from it, without groups once the block has set
+    // itself up.  order_rows_kernel lets this one start when all before it has ended: only who reads its rows waits for it,
+    // the pipeline fills with weights meanwhile.
+    if (a.offsets && !a.ordered) wait_for_previous();
     if (warp == 0) {  // the groups' rows, and the running number of token tiles
         int before = 0, top = a.offsets ? group_offset(a.offsets[0], 0, a.rows) : 0;
         bool bad = a.offsets && top != a.offsets[0];
@@ -406,6 +443,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     let_next_start();
     if constexpr (PAIR) cluster_sync();  // the other block's barriers exist before anything is sent to them
     tc_fence_after();
+    if (!a.offsets || (a.ordered && warp == kRowWarp)) wait_for_previous();
     const uint32_t tmem = *tmem_slot;
     const Groups groups{g_off, g_tiles, a.groups};
     const int tiles_total = g_tiles[a.groups] * a.feat_tiles;
@@ -450,7 +488,6 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
     } else if (warp == kRowWarp) {
         // =========================== rows' producer ===========================
         // Lane j loads the j-th box, with a row index the j-th four rows.
-        if (a.ordered) wait_for_previous();
         const uint32_t full0 = leader_bar(B_FULL);
         uint32_t s = 0, ephase = 1;
         for (int t = unit; t < tiles_total && !timed_out; t += n_units) {
