@@ -73,7 +73,8 @@ int launch_moe_combine(const CombineArgs& a, cudaStream_t stream);
 #ifdef __CUDACC__
 // These kernels follow one another (router, product, product, sum), so each is launched before the one before it has ended
 // (programmatic dependent launch): its blocks start where that one's have left, set themselves up and wait here.  Every thread
-// that reads or writes global memory passes wait_for_previous first; let_next_start comes when a block holds all that it will
+// that reads or writes global memory passes wait_for_previous first (but for the product behind order_rows_kernel, which has
+// waited for it); let_next_start comes when a block holds all that it will
 // ask the SM for, so a waiting successor cannot keep anything from it.  A kernel that does not take part ends before its
 // successor starts.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
