@@ -677,6 +677,35 @@ def test_offsets_past_32_bits():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_grouped_operands_written_right_before():
+    """Weights, offsets, indices and rows that the kernel right before the call has written, where rows are ordered first (the product
+    then starts beside that pass) and where they are gathered."""
+    from llm_compileforge_b200 import ops
+
+    g = gen(52)
+    for rows, experts, ordered in ((2000, 4, 1), (12000, 8, 1), (40, 8, 0)):
+        assert ops.linear_plan(rows, 256, 320, groups=experts, indexed=True)["order"] == ordered
+        versions = []
+        for _ in range(2):
+            x, w = make(g, 300, 256), make(g, experts, 256, 320, std=0.06)
+            offsets = offsets_of(torch.full((rows,), 1.0, device="cuda").multinomial(experts - 1, generator=g).sort().values.diff(
+                prepend=torch.zeros(1, dtype=torch.int64, device="cuda"), append=torch.tensor([rows], device="cuda")).tolist())
+            index = torch.randint(0, 300, (rows,), generator=g, device="cuda", dtype=torch.int32)
+            versions.append(((x, w, offsets, index), ops.grouped_linear(x, w, offsets, row_index=index)))
+            want, tol = linear64(x[index[:1].long()], w[int((offsets <= 0).sum()) - 1])
+            assert_rounded(versions[-1][1][:1], want, tol)
+        torch.cuda.synchronize()
+        now = [torch.empty_like(t) for t in versions[0][0]]
+        for n in range(24):
+            operands, want = versions[n % 2]
+            order = list(range(4))
+            order = order[n % 4:] + order[:n % 4]  # each of them the last one written
+            for i in order:
+                now[i].copy_(operands[i])
+            got = ops.grouped_linear(now[0], now[1], now[2], row_index=now[3])
+            assert torch.equal(got, want), (rows, n)
+
+
 @pytest.mark.parametrize("rows", [3, 200, 700])
 def test_captured_behind_copies_joins_and_at_the_start(rows):
     """Calls as a graph's first node, behind a copy and a fill, beside one another and behind a join of two streams."""
