@@ -90,7 +90,7 @@ def _counts(c):
     for e in rng.choices(range(c["experts"]), weights, k=c["tokens"] * c["top_k"]):
         counts[e] += 1
     if c["skew"]:  # an uneven router leaves experts without a row
-        counts[(counts.index(max(counts)) + 1) % len(counts) or 1] += counts[0]
+        counts[(counts.index(max(counts)) + 1) % len(counts)] += counts[0]
         counts[0] = 0
     return counts
 
