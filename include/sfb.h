@@ -505,7 +505,7 @@ SFB_API int sfb_linear_plan(int64_t rows, int64_t K, int64_t N, int64_t groups, 
  * weights: softmax over the chosen experts (renormalize) or over all E.  Assignment (t, j) is row positions[t, j] of the
  * sorted order, token_rows[row] = t, rows of expert e are group_offsets[e] .. group_offsets[e + 1] in the order of
  * tokens; token_rows behind the last row is -1.  (logits of +inf share the weight among themselves.)
- * workspace: sfb_moe_route_workspace_bytes(T, E) bytes, 0 for few tokens; its contents need not be kept. */
+ * workspace: sfb_moe_route_workspace_bytes(T, E) bytes, 4-byte aligned, 0 for few tokens; its contents need not be kept. */
 SFB_API int64_t sfb_moe_route_workspace_bytes(int64_t tokens, int64_t experts);
 SFB_API int sfb_moe_route(const SFBTensor* logits, SFBTensor* expert_ids, SFBTensor* weights, SFBTensor* group_offsets, SFBTensor* token_rows,
                           SFBTensor* positions, int dtype, int renormalize, void* workspace, int64_t workspace_bytes, void* stream);

@@ -212,6 +212,7 @@ int sfb_moe_route(const SFBTensor* logits, SFBTensor* expert_ids, SFBTensor* wei
     const int64_t need = sfb_moe_route_workspace_bytes(T, E);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(SFB_ERR_WORKSPACE, "moe_route: workspace of %lld B needed, %lld given", (long long)need, (long long)(workspace ? workspace_bytes : 0));
+    if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 4) return fail(SFB_ERR_INVALID_ARG, "moe_route: workspace must start on 4 bytes (int32 counts)");
     RouteArgs a{};
     a.logits = vl.base; a.logits_stride = vl.stride[2];
     a.ids = reinterpret_cast<int32_t*>(vi.base); a.weights = reinterpret_cast<float*>(vw.base);

@@ -661,7 +661,7 @@ class MoeRouting(NamedTuple):
 def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, workspace: torch.Tensor | None = None) -> MoeRouting:
     """The ``top_k`` experts of every token (``logits [T, E]``; larger logit first, then lower index), their softmax weights
     over the chosen experts (``renormalize``) or over all, and the assignments sorted by expert, then token.  A logit of
-    ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8,
+    ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8, on 4 bytes,
     :func:`moe_route_workspace_bytes`) is allocated when missing."""
     got = _quick("route")(logits, top_k, renormalize, workspace)
     if got is not None:

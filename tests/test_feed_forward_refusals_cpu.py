@@ -1,0 +1,27 @@
+"""More refusals of the feed-forward operators, without a GPU: every call here ends before a launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+from llm_compileforge_b200 import B200Backend, _lib, ops
+from test_abi_cpu import _fake_desc
+
+TOKENS, EXPERTS, TOP = 300, 16, 2
+
+
+def route(workspace, n_bytes):
+    lib = _lib.load()
+    descs = [_fake_desc((TOKENS, EXPERTS), 4), _fake_desc((TOKENS, TOP), 4), _fake_desc((TOKENS, TOP), 4), _fake_desc((EXPERTS + 1,), 4),
+             _fake_desc((TOKENS * TOP,), 4), _fake_desc((TOKENS, TOP), 4)]
+    return lib.sfb_moe_route(*(ctypes.cast(ctypes.pointer(d), ctypes.c_void_p) for d in descs), _lib.SFB_F32, 1, workspace, n_bytes, None)
+
+
+@pytest.mark.parametrize("odd", [1, 2, 3, 5])
+def test_route_workspace_off_four_bytes_is_refused(odd):
+    need = ops.moe_route_workspace_bytes(TOKENS, EXPERTS)
+    assert need > 0
+    assert route(0x10000 + odd, need) == _lib.SFB_ERR_INVALID_ARG
+    assert "4 bytes" in _lib.load().sfb_last_error().decode()
+    assert route(0x10000 + odd, need - 1) == _lib.SFB_ERR_WORKSPACE
