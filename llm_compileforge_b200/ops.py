@@ -582,6 +582,8 @@ def _workspace(what: str, workspace: torch.Tensor | None, need: int, like: torch
         workspace = like.new_empty(need, dtype=torch.uint8)
     elif workspace.get_device() != like.get_device():
         raise ValueError(f"{what}: workspace on {workspace.device}, operands on {like.device}")
+    elif not workspace.is_contiguous():  # its size below is that of its elements only where they lie side by side
+        raise ValueError(f"{what}: workspace must be contiguous, strides {workspace.stride()}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 

@@ -25,3 +25,13 @@ def test_route_workspace_off_four_bytes_is_refused(odd):
     assert route(0x10000 + odd, need) == _lib.SFB_ERR_INVALID_ARG
     assert "4 bytes" in _lib.load().sfb_last_error().decode()
     assert route(0x10000 + odd, need - 1) == _lib.SFB_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2],
+                                       torch.zeros(1024, 512, dtype=torch.uint8).t()])
+def test_workspaces_that_are_not_one_piece_are_refused(workspace):
+    x, w, index = torch.zeros(64, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16), torch.zeros(64, dtype=torch.int32)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.moe_route(torch.zeros(TOKENS, EXPERTS), TOP, workspace=workspace)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.grouped_linear(x, w, torch.zeros(3, dtype=torch.int32), row_index=index, workspace=workspace)
