@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import threading
 from ctypes import POINTER, Structure, Union, byref, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
@@ -84,6 +85,7 @@ class SfbError(RuntimeError):
 
 
 _lib: ctypes.CDLL | None = None
+_loading = threading.Lock()
 
 _T = POINTER(SFBTensor)
 
@@ -91,8 +93,16 @@ _T = POINTER(SFBTensor)
 def load() -> ctypes.CDLL:
     """Load libsfb.so; raises ``RuntimeError`` when it has not been built."""
     global _lib
-    if _lib is not None:
-        return _lib
+    if _lib is None:
+        with _loading:
+            if _lib is None:
+                lib = _open()
+                _bind_calls(lib)
+                _lib = lib  # last: whoever finds it set finds all of it
+    return _lib
+
+
+def _open() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(
             f"{LIB_PATH} is missing: build it with `python -m llm_compileforge_b200.build` "
@@ -138,8 +148,6 @@ def load() -> ctypes.CDLL:
     lib.sfb_fused_rms_norm_matmul_plan.argtypes = [c_int64, c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int32)]
     lib.sfb_peer_signal_wait.restype = c_int
     lib.sfb_peer_signal_wait.argtypes = [POINTER(c_void_p), c_int, c_int, ctypes.c_uint32, c_int, c_void_p, c_void_p]
-    _lib = lib
-    _bind_calls(lib)
     return lib
 
 
