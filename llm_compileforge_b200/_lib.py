@@ -11,6 +11,7 @@ import ctypes
 import os
 import struct
 import threading
+import warnings
 from ctypes import POINTER, Structure, Union, byref, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
@@ -152,7 +153,7 @@ def _open() -> ctypes.CDLL:
 
 
 class _NoCalls:
-    """Stands in for the ``_calls`` module where it is not built: no call is one of its."""
+    """Stands in for the ``_calls`` module where there is none for this torch: no call is one of its."""
 
     @staticmethod
     def linear(*args):
@@ -166,10 +167,18 @@ calls = None  # the quick way into the library (csrc/calls.cpp), set when the li
 
 def _bind_calls(lib: ctypes.CDLL) -> None:
     global calls
+    calls = _NoCalls
     try:
         from . import _calls
     except ModuleNotFoundError:
-        calls = _NoCalls
+        return
+    except ImportError as e:  # built against another torch or Python, as a rule
+        warnings.warn(f"the extension module _calls does not load ({e}): rebuild it with `python -m llm_compileforge_b200.build`", RuntimeWarning, stacklevel=3)
+        return
+    built_for = getattr(_calls, "torch_version", "of an unknown version")
+    if built_for != torch.__version__:  # it takes tensors apart by that torch's headers
+        warnings.warn(f"the extension module _calls was built for torch {built_for}, this is {torch.__version__}: "
+                      "rebuild it with `python -m llm_compileforge_b200.build`", RuntimeWarning, stacklevel=3)
         return
     names = ("sfb_fused_linear", "sfb_grouped_linear", "sfb_grouped_linear_workspace_bytes", "sfb_moe_route", "sfb_moe_route_workspace_bytes", "sfb_moe_combine")
     _calls.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in names))

@@ -97,6 +97,7 @@ def build_calls(force: bool, run) -> None:
 
     include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         f'-DSFB_TORCH_VERSION="{torch.__version__}"',
          *(f"-I{d}" for d in include), src, "-o", out, *(f"-L{d}" for d in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
 
 

@@ -306,4 +306,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", SFB_TORCH_VERSION) < 0) Py_CLEAR(m);  // of the headers above
+    return m;
+}

@@ -1,10 +1,15 @@
 """How the library and its extension module are loaded, without a GPU."""
 
+import sys
 import threading
+import types
+import warnings
 
 import pytest
+import torch
 
-from llm_compileforge_b200 import _lib
+import llm_compileforge_b200 as package
+from llm_compileforge_b200 import _lib, ops
 
 
 @pytest.fixture
@@ -52,3 +57,56 @@ def test_a_load_that_fails_is_tried_again(unloaded):
                 _lib.load()
     _lib.load()
     assert _lib.calls is not None
+
+
+class Broken:
+    """A finder for which the extension module is there but does not load."""
+
+    def find_spec(self, name, path=None, target=None):
+        if name.endswith("._calls"):
+            raise ImportError("undefined symbol: _ZN3c10")
+
+
+@pytest.fixture
+def without_module(unloaded):
+    unloaded.delattr(package, "_calls", raising=False)
+    unloaded.delitem(sys.modules, package.__name__ + "._calls", raising=False)
+    return unloaded
+
+
+def bad_call_in_words():
+    with pytest.raises(ValueError, match="K is zero"):
+        ops.fused_linear(torch.zeros(4, 0), torch.zeros(0, 8))
+
+
+def test_a_module_that_does_not_load_leaves_the_other_way(without_module):
+    without_module.setattr(sys, "meta_path", [Broken(), *sys.meta_path])
+    with pytest.warns(RuntimeWarning, match="undefined symbol.*build"):
+        _lib.load()
+    bad_call_in_words()
+
+
+def test_a_module_that_is_not_built_leaves_the_other_way(without_module):
+    class Absent(Broken):
+        def find_spec(self, name, path=None, target=None):
+            if name.endswith("._calls"):
+                raise ModuleNotFoundError(name)
+
+    without_module.setattr(sys, "meta_path", [Absent(), *sys.meta_path])
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        _lib.load()
+    bad_call_in_words()
+
+
+def test_a_module_of_another_torch_is_not_used(unloaded):
+    unloaded.setattr(package, "_calls", types.SimpleNamespace(torch_version="1.0", bind=lambda *a: pytest.fail("bound")), raising=False)
+    with pytest.warns(RuntimeWarning, match="1.0.*build"):
+        _lib.load()
+    bad_call_in_words()
+
+
+def test_the_built_module_names_its_torch():
+    from llm_compileforge_b200 import _calls
+
+    assert _calls.torch_version == torch.__version__
