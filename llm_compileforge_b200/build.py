@@ -89,16 +89,23 @@ def calls_path() -> str:
 
 
 def build_calls(force: bool, run) -> None:
-    src, out = os.path.join(CSRC, "calls.cpp"), calls_path()
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), _headers_mtime()):
-        return
+    """The extension module, for the torch that is installed: it is built again when that changes."""
     import torch
     from torch.utils import cpp_extension
 
+    src, out, note = os.path.join(CSRC, "calls.cpp"), calls_path(), os.path.join(OBJ, "_calls.torch")
+    built_for = None
+    if os.path.exists(out) and os.path.exists(note):
+        with open(note) as f:
+            built_for = f.read()
+    if not force and built_for == torch.__version__ and os.path.getmtime(out) >= max(os.path.getmtime(src), _headers_mtime()):
+        return
     include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
          f'-DSFB_TORCH_VERSION="{torch.__version__}"',
          *(f"-I{d}" for d in include), src, "-o", out, *(f"-L{d}" for d in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    with open(note, "w") as f:
+        f.write(torch.__version__)
 
 
 if __name__ == "__main__":

@@ -1,5 +1,6 @@
 """How the library and its extension module are loaded, without a GPU."""
 
+import os
 import sys
 import threading
 import types
@@ -9,7 +10,7 @@ import pytest
 import torch
 
 import llm_compileforge_b200 as package
-from llm_compileforge_b200 import _lib, ops
+from llm_compileforge_b200 import _lib, build, ops
 
 
 @pytest.fixture
@@ -110,3 +111,25 @@ def test_the_built_module_names_its_torch():
     from llm_compileforge_b200 import _calls
 
     assert _calls.torch_version == torch.__version__
+
+
+@pytest.fixture
+def calls_build(monkeypatch, tmp_path):
+    """build.build_calls into an empty folder, the compiler replaced by one that notes its commands and writes its output."""
+    commands = []
+
+    def run(cmd):
+        commands.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("built")
+
+    monkeypatch.setattr(build, "calls_path", lambda: str(tmp_path / "_calls.so"))
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    return lambda force=False: (build.build_calls(force, run), len(commands), os.path.exists(tmp_path / "_calls.so"))[1:]
+
+
+def test_the_module_is_built_again_for_another_torch(calls_build, monkeypatch):
+    assert calls_build() == (1, True) and calls_build() == (1, True)
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    assert calls_build() == (2, True) and calls_build() == (2, True)
+    assert calls_build(force=True) == (3, True)
