@@ -12,6 +12,7 @@ against PyTorch's headers: the quick way from Python into the library).
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -89,10 +90,14 @@ def calls_path() -> str:
 
 
 def build_calls(force: bool, run) -> None:
-    """The extension module, for the torch that is installed: it is built again when that changes."""
-    import torch
-    from torch.utils import cpp_extension
-
+    """The extension module, for the torch that is installed: it is built again when that changes.  Where torch, its or Python's
+    headers or a C++ compiler are missing there is none, and the library, which needs none of them, stands by itself."""
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError as e:
+        sys.stderr.write(f"no extension module _calls: torch does not import ({e})\n")
+        return
     src, out, note = os.path.join(CSRC, "calls.cpp"), calls_path(), os.path.join(OBJ, "_calls.torch")
     built_for = None
     if os.path.exists(out) and os.path.exists(note):
@@ -101,6 +106,12 @@ def build_calls(force: bool, run) -> None:
     if not force and built_for == torch.__version__ and os.path.getmtime(out) >= max(os.path.getmtime(src), _headers_mtime()):
         return
     include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    missing = [h for h in ("torch/csrc/autograd/python_variable.h", "Python.h") if not any(os.path.exists(os.path.join(d, h)) for d in include)]
+    if missing or not shutil.which("g++"):
+        sys.stderr.write(f"no extension module _calls: {f'headers missing ({missing[0]})' if missing else 'no g++'}\n")
+        if built_for != torch.__version__ and os.path.exists(out):
+            os.remove(out)  # of another torch
+        return
     run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
          f'-DSFB_TORCH_VERSION="{torch.__version__}"',
          *(f"-I{d}" for d in include), src, "-o", out, *(f"-L{d}" for d in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])

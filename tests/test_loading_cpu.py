@@ -133,3 +133,20 @@ def test_the_module_is_built_again_for_another_torch(calls_build, monkeypatch):
     monkeypatch.setattr(torch, "__version__", "99.0")
     assert calls_build() == (2, True) and calls_build() == (2, True)
     assert calls_build(force=True) == (3, True)
+
+
+def test_without_torch_headers_the_library_is_built_all_the_same(calls_build, monkeypatch, tmp_path, capsys):
+    from torch.utils import cpp_extension
+
+    assert calls_build() == (1, True)
+    monkeypatch.setattr(cpp_extension, "include_paths", lambda *a, **k: [str(tmp_path)])
+    assert calls_build() == (1, True)  # still the one for this torch
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    assert calls_build() == (1, False)  # the one for another torch does not stay
+    assert "headers" in capsys.readouterr().err
+
+
+def test_without_torch_the_library_is_built_all_the_same(calls_build, monkeypatch, capsys):
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert calls_build() == (0, False)
+    assert "torch" in capsys.readouterr().err
