@@ -468,7 +468,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
                 const int n0 = column0(tile), n1 = n0 + (a.gated ? 0 : 64);
                 for (int k = k_first; k < k_end; k += sub) {
-                    if (!mbar_wait(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
+                    if (!mbar_wait<PAIR>(bar(B_EMPTY + s), ephase)) { timed_out = true; break; }
                     const int end = min(k + (int)sub, k_end);
                     if (!PAIR || rank == 0) mbar_expect_tx(bar(B_FULL + s), (end - k) * bytes);
                     const uint32_t full = full0 + 8 * s;
@@ -482,7 +482,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
             // the leader's commits arrive in both blocks: none may still be under way when this one leaves
             for (uint32_t i = 0; PAIR && i < stages && !timed_out; ++i) {
-                timed_out = !mbar_wait(bar(B_EMPTY + s), ephase);
+                timed_out = !mbar_wait<PAIR>(bar(B_EMPTY + s), ephase);
                 if (++s == stages) { s = 0; ephase ^= 1; }
             }
         }
@@ -514,7 +514,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
             }
             for (int k = k_first; k < k_end; k += sub) {
                 // (all lanes step together: one without a box that fell behind would miss a phase that it waits for)
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(B_EMPTY + s), ephase))) { timed_out = true; break; }
+                if (!__all_sync(0xffffffffu, mbar_wait<PAIR>(bar(B_EMPTY + s), ephase))) { timed_out = true; break; }
                 const int end = min(k + (int)sub, k_end);
                 if (lane == 0 && (!PAIR || rank == 0)) mbar_expect_tx(bar(B_FULL + s), (end - k) * bytes);
                 uint32_t dst = place + s * stage_bytes;
@@ -539,7 +539,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
                 const Tile tile = groups.at(t, a.feat_tiles, a.block, S::kRound);
                 const uint32_t idesc = instr_desc(BF16, !a.nk, PAIR ? 2 * kFeat : kFeat, (tile.rows + S::kRound - 1) / S::kRound * S::kRound);
                 const int buf = it & 1;
-                ok = mbar_wait(bar(B_ACC_EMPTY + buf), ((it >> 1) & 1) ^ 1);
+                ok = mbar_wait<PAIR>(bar(B_ACC_EMPTY + buf), ((it >> 1) & 1) ^ 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * kTok;
