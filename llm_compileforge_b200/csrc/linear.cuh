@@ -108,7 +108,7 @@ __device__ __forceinline__ void settle() {
 __device__ __forceinline__ int group_offset(int raw, int before, int rows) { return max(before, min(raw, rows)); }
 
 // The activations in fp32.  silu and the tanh form of gelu as h * logistic(.), the erf form as h/2 * erfc(-h / sqrt 2):
-// none of them subtracts nearly equal numbers for large negative h.
+// none of them subtracts nearly equal numbers for large negative h.  (On the tensor cores: activate_all in linear_tcgen05.cu.)
 template <int ACT>
 __device__ __forceinline__ float activate(float h) {
     if constexpr (ACT == SFB_ACT_SILU) return h / (1.f + __expf(-h));

@@ -313,18 +313,20 @@ __device__ __forceinline__ float exp2_approx(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// h Phi(h), two at a time: Phi(-x) = 2^P(x), P the polynomial of degree 8 that fits log2 Phi(-x) on [0, 13.2] best under the
-// weight max(x, 1/2) Phi(-x) + 1e-8 (Lawson's iteration); |h| Phi(-|h|) comes out within 1.7e-7 |h|, and P(13.2) = -136 makes it
-// zero from there on.  One exponential and ten multiply-adds: the tile's epilogue is bound by the FMA pipes.  A
+// h Phi(h), two at a time: Phi(-x) = 2^P(x), P the polynomial of degree 11 that fits log2 Phi(-x) on [0, 13.2] best where 2^P may
+// be off by the smaller of 2^-12 of itself and 6e-8 (Lawson's iteration).  With the rounding of its terms and of ex2 h Phi(h) comes
+// out within 3e-7 |h|, and for -12.9 <= h < 0 within 2^-11 of itself, a quarter of bf16's half step and less above -6; below, where
+// Phi is no normal number, it is zero.  One exponential and thirteen multiply-adds: the tile's epilogue is bound by the FMA pipes.  A
 // [1001, 2048] x [2048, 8192] product took 34.3 us with a fit of one exponential, one division and one value at a time, 32.2 with
-// exp(-x^2 / 2) times a polynomial of degree 11, 31.2 with this; with erfcf the epilogue alone took four times the MMAs.
+// exp(-x^2 / 2) times a polynomial of degree 11; measured in turn, 32.1 with a polynomial of degree 8 (22 % off at h = -7) and 32.5
+// with this; with erfcf the epilogue alone took four times the MMAs.
 __device__ __forceinline__ void gelu_erf(float& a, float& b) {
-    constexpr float c[9] = {-9.999997698e-01f, -1.151117087e+00f, -4.591095006e-01f, -5.279575703e-02f, 7.495873251e-03f,
-                            -4.663810760e-04f, -5.088244300e-05f, 1.120313268e-05f, -5.128124838e-07f};
+    constexpr float c[12] = {-9.999998212e-01f, -1.151115060e+00f, -4.591248930e-01f, -5.274898559e-02f, 7.415628992e-03f, -3.830976493e-04f,
+                             -1.012203720e-04f, 2.793559543e-05f, -3.357467222e-06f, 2.251555600e-07f, -8.138483665e-09f, 1.236985236e-10f};
     const Two x(fminf(fabsf(a), 13.2f), fminf(fabsf(b), 13.2f));
-    Two p(c[8]);
+    Two p(c[11]);
 #pragma unroll
-    for (int i = 7; i >= 0; --i) p = fma2(p, x, Two(c[i]));
+    for (int i = 10; i >= 0; --i) p = fma2(p, x, Two(c[i]));
     const float2 e = p.get();
     const Two q(exp2_approx(e.x), exp2_approx(e.y));
     const float2 lo = q.get(), hi = fma2(q, Two(-1.f), Two(1.f)).get();
