@@ -107,13 +107,23 @@ __device__ __forceinline__ void settle() {
 // counts as that one.  Groups then never overlap or leave the rows, whatever the array holds.
 __device__ __forceinline__ int group_offset(int raw, int before, int rows) { return max(before, min(raw, rows)); }
 
+// 1 / (1 + 2^t) from t - 8.  The sum is formed 2^8 smaller than it is: its reciprocal then stays a normal number until t = 134, and
+// h / (1 + 2^t), h itself some ten to ninety, until it is none itself (unscaled it became zero from t = 126 on).
+__device__ __forceinline__ float logistic_exp2(float t_minus_8) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t_minus_8));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 0x1p-8f));
+    return r * 0x1p-8f;
+}
+constexpr float kLog2E = 1.4426950408889634f, kTanhGelu = 1.5957691216057308f;  // log2 e, 2 sqrt(2 / pi)
+
 // The activations in fp32.  silu and the tanh form of gelu as h * logistic(.), the erf form as h/2 * erfc(-h / sqrt 2):
-// none of them subtracts nearly equal numbers for large negative h.  (On the tensor cores: activate_all in linear_tcgen05.cu.)
+// none of them subtracts nearly equal numbers for large negative h.  (The erf form on the tensor cores: linear_tcgen05.cu.)
 template <int ACT>
 __device__ __forceinline__ float activate(float h) {
-    if constexpr (ACT == SFB_ACT_SILU) return h / (1.f + __expf(-h));
+    if constexpr (ACT == SFB_ACT_SILU) return h * logistic_exp2(fmaf(h, -kLog2E, -8.f));
     if constexpr (ACT == SFB_ACT_GELU) return 0.5f * h * erfcf(-0.70710678118654752f * h);
-    if constexpr (ACT == SFB_ACT_GELU_TANH) return h / (1.f + __expf(-1.5957691216057308f * (h + 0.044715f * h * h * h)));
+    if constexpr (ACT == SFB_ACT_GELU_TANH) return h * logistic_exp2(fmaf(h, fmaf(h * h, -kLog2E * kTanhGelu * 0.044715f, -kLog2E * kTanhGelu), -8.f));
     if constexpr (ACT == SFB_ACT_RELU) return h < 0.f ? 0.f : h;
     return h;
 }

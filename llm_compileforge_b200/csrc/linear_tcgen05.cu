@@ -340,12 +340,12 @@ __device__ __forceinline__ void activate_all(float (&h)[W], int act) {
 #pragma unroll
         for (int i = 0; i < W; ++i) h[i] = f(h[i]);
     };
-    if (act == SFB_ACT_SILU) each([](float v) { return __fdividef(v, 1.f + __expf(-v)); });
+    if (act == SFB_ACT_SILU) each([](float v) { return activate<SFB_ACT_SILU>(v); });
     else if (act == SFB_ACT_GELU) {
 #pragma unroll
         for (int i = 0; i < W; i += 2) gelu_erf(h[i], h[i + 1]);
     }
-    else if (act == SFB_ACT_GELU_TANH) each([](float v) { return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v))); });
+    else if (act == SFB_ACT_GELU_TANH) each([](float v) { return activate<SFB_ACT_GELU_TANH>(v); });
     else if (act == SFB_ACT_RELU) each([](float v) { return activate<SFB_ACT_RELU>(v); });
 }
 

@@ -67,3 +67,25 @@ def test_erf_gelu_over_its_range(form, dtype, out_dtype):
     far = torch.tensor([-13.5, -20.0, -3e4, 20.0, 3e4], dtype=dtype, device="cuda")
     got = act_alone(far.repeat(800), form, "gelu", out_dtype).double()[:5]
     assert (got[:3].abs() < 1e-38).all() and (got[3:] == far[3:].double()).all()
+
+
+@pytest.mark.parametrize("out_dtype", [None, torch.float32])
+@pytest.mark.parametrize("form", FORMS)
+def test_silu_and_tanh_gelu_as_far_as_they_are_normal_numbers(form, out_dtype):
+    """h / (1 + 2^t) in fp32: what t is off by, times ln 2, is the result's relative error.  silu, t = -h log2 e up to 132: half a step
+    of t (2^-18) and the constant's 1.3e-8 of it, 4e-6 with the rest below 2^-17; from t = 126 on the logistic is a subnormal number of at
+    least 15 bits, 2^-16 more.  tanh gelu, t up to 133: two roundings and a constant more, 2.5 steps of 2^-24 of t, 1.7e-5, and the same
+    2^-16: below 2^-14."""
+    h = values(-91.5, 30, BF16)
+    tol = torch.where(h > -87, 2.0 ** -17, 2.0 ** -15)
+    want = h.double() * torch.special.expit(h.double())
+    assert_rounded(act_alone(h, form, "silu", out_dtype), want, want.abs() * tol, form)
+    h = values(-10.0625, 10, BF16)
+    d = h.double()
+    want = d * torch.special.expit(2 * (2 / torch.pi) ** 0.5 * (d + 0.044715 * d ** 3))
+    assert_rounded(act_alone(h, form, "gelu_tanh", out_dtype), want, want.abs() * 2.0 ** -14, form)
+    far = torch.tensor([-3e38, -1e4, 1e-37, -1e-37, 1e4, 3e38], dtype=BF16, device="cuda")
+    for act in ("silu", "gelu_tanh"):
+        got = act_alone(far.repeat(800), form, act, out_dtype).double()[:6]
+        assert (got[:2] == 0).all() and (got[4:] == far[4:].double()).all()
+        assert ((got[2:4] - far[2:4].double() / 2).abs() <= 2.0 ** -8 * 1e-37).all()
