@@ -43,6 +43,11 @@ except Exception:  # noqa: BLE001
             raise NotImplementedError("send_kv_cache not supported")
 
 
+def _count(op: str, inputs: list[Any], least: int, most: int) -> None:
+    if not least <= len(inputs) <= most:
+        raise ValueError(f"{op}: {least if least == most else f'{least} to {most}'} inputs, got {len(inputs)} (the rest are keywords)")
+
+
 class B200Backend(OpExecutor):
     """Attention hot-path operators on one B200.
 
@@ -254,19 +259,23 @@ class B200Backend(OpExecutor):
 
     def _op_fused_linear(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[x, weight(, bias)]`` with the keywords of :func:`ops.fused_linear`."""
-        return ops.fused_linear(*inputs[:3], **kw)
+        _count("fused_linear", inputs, 2, 3)
+        return ops.fused_linear(*inputs, **kw)
 
     def _op_grouped_linear(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[x, weight, group_offsets(, bias)]`` with the keywords of :func:`ops.grouped_linear`."""
-        return ops.grouped_linear(*inputs[:4], **kw)
+        _count("grouped_linear", inputs, 3, 4)
+        return ops.grouped_linear(*inputs, **kw)
 
     def _op_moe_route(self, inputs: list[Any], **kw: Any) -> Any:
         """inputs ``[logits]`` with ``top_k`` and the keywords of :func:`ops.moe_route`."""
+        _count("moe_route", inputs, 1, 1)
         return ops.moe_route(inputs[0], kw.pop("top_k"), **kw)
 
     def _op_moe_combine(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[y, positions, weights]`` with the keywords of :func:`ops.moe_combine`."""
-        return ops.moe_combine(*inputs[:3], **kw)
+        _count("moe_combine", inputs, 3, 3)
+        return ops.moe_combine(*inputs, **kw)
 
     def _op_chunked_prefill(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[query [T,H,D], key_cache, value_cache, block_table [R,max_blocks]]``

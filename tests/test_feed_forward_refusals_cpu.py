@@ -35,3 +35,13 @@ def test_workspaces_that_are_not_one_piece_are_refused(workspace):
         ops.moe_route(torch.zeros(TOKENS, EXPERTS), TOP, workspace=workspace)
     with pytest.raises(ValueError, match="contiguous"):
         ops.grouped_linear(x, w, torch.zeros(3, dtype=torch.int32), row_index=index, workspace=workspace)
+
+
+def test_executor_refuses_operands_that_it_does_not_take():
+    hal = B200Backend()
+    x, w, b, r = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8), torch.zeros(4, 8)
+    i = torch.zeros(4, 2, dtype=torch.int32)
+    for name, inputs in (("fused_linear", [x, w, b, r]), ("fused_linear", [x]), ("grouped_linear", [x, w[None], i[0], b[None], w[None]]), ("grouped_linear", [x, w[None]]),
+                         ("moe_route", [x, x]), ("moe_route", []), ("moe_combine", [x, i, torch.zeros(4, 2), r]), ("moe_combine", [x, i])):
+        with pytest.raises(ValueError, match=f"{name}: .* inputs"):
+            hal.execute(name, inputs, **({"top_k": 2} if name == "moe_route" else {}))
