@@ -270,7 +270,9 @@ class B200Backend(OpExecutor):
     def _op_moe_route(self, inputs: list[Any], **kw: Any) -> Any:
         """inputs ``[logits]`` with ``top_k`` and the keywords of :func:`ops.moe_route`."""
         _count("moe_route", inputs, 1, 1)
-        return ops.moe_route(inputs[0], kw.pop("top_k"), **kw)
+        if "top_k" not in kw:
+            raise ValueError("moe_route needs top_k")
+        return ops.moe_route(inputs[0], **kw)
 
     def _op_moe_combine(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         """inputs ``[y, positions, weights]`` with the keywords of :func:`ops.moe_combine`."""

@@ -45,3 +45,8 @@ def test_executor_refuses_operands_that_it_does_not_take():
                          ("moe_route", [x, x]), ("moe_route", []), ("moe_combine", [x, i, torch.zeros(4, 2), r]), ("moe_combine", [x, i])):
         with pytest.raises(ValueError, match=f"{name}: .* inputs"):
             hal.execute(name, inputs, **({"top_k": 2} if name == "moe_route" else {}))
+
+
+def test_executor_asks_for_top_k():
+    with pytest.raises(ValueError, match="top_k"):
+        B200Backend().execute("moe_route", [torch.zeros(4, 8)])
