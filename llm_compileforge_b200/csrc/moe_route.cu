@@ -12,7 +12,9 @@
 // of the atomics.
 // With at most 128 tokens one launch does everything; with more, a second launch adds up the blocks' counts and places the
 // rows (from 256 blocks up, where every block adding all counts would be quadratic, a scan comes in between).
-// Bound: launch latency for few tokens, the selection rounds' instructions for many.
+// Bound: launch latency for few tokens.  Many take two dependent launches, of 16384 tokens of 128 experts 11.4 and 7.7 us (of 256 15.3
+// and 9.7; each by itself, caches cold), where the bytes would take 1: a block per 128 tokens fills 128 of 148 SMs once, and the second
+// launch reads the choices back and adds every block's counts.  The selection's instructions, about 200 a token and warp, are 3 to 4 us of it.
 
 #include <algorithm>
 #include <type_traits>
