@@ -109,8 +109,8 @@ def build_calls(force: bool, run) -> None:
     missing = [h for h in ("torch/csrc/autograd/python_variable.h", "Python.h") if not any(os.path.exists(os.path.join(d, h)) for d in include)]
     if missing or not shutil.which("g++"):
         sys.stderr.write(f"no extension module _calls: {f'headers missing ({missing[0]})' if missing else 'no g++'}\n")
-        if built_for != torch.__version__ and os.path.exists(out):
-            os.remove(out)  # of another torch
+        if os.path.exists(out):
+            os.remove(out)  # of another torch, or older than its sources
         return
     run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
          f'-DSFB_TORCH_VERSION="{torch.__version__}"',

@@ -146,6 +146,14 @@ def test_without_torch_headers_the_library_is_built_all_the_same(calls_build, mo
     assert "headers" in capsys.readouterr().err
 
 
+def test_without_a_compiler_no_module_older_than_its_sources_stays(calls_build, monkeypatch):
+    assert calls_build() == (1, True)
+    monkeypatch.setattr(build.shutil, "which", lambda name: None)
+    assert calls_build() == (1, True)
+    monkeypatch.setattr(build, "_headers_mtime", lambda: 1e12)  # the C ABI that it was built against is another now
+    assert calls_build() == (1, False)
+
+
 def test_without_torch_the_library_is_built_all_the_same(calls_build, monkeypatch, capsys):
     monkeypatch.setitem(sys.modules, "torch", None)
     assert calls_build() == (0, False)
