@@ -115,15 +115,15 @@ __device__ __forceinline__ float logistic_exp2(float t_minus_8) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 0x1p-8f));
     return r * 0x1p-8f;
 }
-constexpr float kLog2E = 1.4426950408889634f, kTanhGelu = 1.5957691216057308f;  // log2 e, 2 sqrt(2 / pi)
+constexpr double kLog2E = 1.4426950408889634, kTanhGelu = 1.5957691216057308 * kLog2E;  // log2 e, 2 sqrt(2 / pi) log2 e
 
 // The activations in fp32.  silu and the tanh form of gelu as h * logistic(.), the erf form as h/2 * erfc(-h / sqrt 2):
 // none of them subtracts nearly equal numbers for large negative h.  (The erf form on the tensor cores: linear_tcgen05.cu.)
 template <int ACT>
 __device__ __forceinline__ float activate(float h) {
-    if constexpr (ACT == SFB_ACT_SILU) return h * logistic_exp2(fmaf(h, -kLog2E, -8.f));
+    if constexpr (ACT == SFB_ACT_SILU) return h * logistic_exp2(fmaf(h, (float)-kLog2E, -8.f));
     if constexpr (ACT == SFB_ACT_GELU) return 0.5f * h * erfcf(-0.70710678118654752f * h);
-    if constexpr (ACT == SFB_ACT_GELU_TANH) return h * logistic_exp2(fmaf(h, fmaf(h * h, -kLog2E * kTanhGelu * 0.044715f, -kLog2E * kTanhGelu), -8.f));
+    if constexpr (ACT == SFB_ACT_GELU_TANH) return h * logistic_exp2(fmaf(h, fmaf(h * h, (float)(-kTanhGelu * 0.044715), (float)-kTanhGelu), -8.f));
     if constexpr (ACT == SFB_ACT_RELU) return h < 0.f ? 0.f : h;
     return h;
 }

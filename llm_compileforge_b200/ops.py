@@ -596,7 +596,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_offsets: torch.T
     ``[E + 1]``, read on the device, groups may be empty) is ``act(x[i] @ weight[e] + bias[e]) * (x[i] @ up_weight[e] + up_bias[e])``
     with ``i = row_index[r]`` (int32, one entry per row of the result) or ``i = r`` without one.  ``weight`` and ``up_weight``
     ``[E, K, N]`` with either of the last two dimensions contiguous, biases ``[E, N]``.  Rows outside every group are left as
-    they were (in a fresh result: undefined).  ``out`` shares memory with no operand.  ``workspace`` (uint8,
+    they were (in a fresh result: undefined).  ``out`` shares memory with no operand.  ``workspace`` (uint8, contiguous,
     :func:`grouped_linear_workspace_bytes`; allocated when missing) holds the rows of ``x`` in the order of ``row_index`` where groups
     have many.  ``status`` (int32, device) collects ``SFB_STATUS_BAD_ROW_INDEX`` for offsets or indices outside their range."""
     if type(activation) is str and (out_dtype is None or out_dtype is torch.float32):
@@ -664,7 +664,7 @@ class MoeRouting(NamedTuple):
 def moe_route(logits: torch.Tensor, top_k: int, *, renormalize: bool = True, workspace: torch.Tensor | None = None) -> MoeRouting:
     """The ``top_k`` experts of every token (``logits [T, E]``; larger logit first, then lower index), their softmax weights
     over the chosen experts (``renormalize``) or over all, and the assignments sorted by expert, then token.  A logit of
-    ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8, on 4 bytes,
+    ``-inf`` or NaN never chooses its expert, so rows that pad a batch are given ``-inf`` throughout.  ``workspace`` (uint8, contiguous, on 4 bytes,
     :func:`moe_route_workspace_bytes`) is allocated when missing."""
     got = _quick("route")(logits, top_k, renormalize, workspace)
     if got is not None:
